@@ -21,7 +21,7 @@ PRODUCT_LIB_PATH = os.path.join(_HERE, "libiffnerf_hip.so")
 LIB_PATH = os.environ.get("IFF_LIB_PATH") or PRODUCT_LIB_PATH
 DEV_LIBRARY = os.path.abspath(LIB_PATH) != os.path.abspath(PRODUCT_LIB_PATH)
 _lib = None
-ABI_VERSION = 12         # include/iffnerf_hip.h IFF_ABI_VERSION this binding was written against
+ABI_VERSION = 13         # include/iffnerf_hip.h IFF_ABI_VERSION this binding was written against
 
 c_float_p = C.POINTER(C.c_float)
 
@@ -57,6 +57,8 @@ class VitDesc(C.Structure):
 
 
 VIT_FP32, VIT_BF16 = 0, 1          # include/iffnerf_hip.h IFF_VIT_FP32 / IFF_VIT_BF16
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # IFF_TYPE_F32 / IFF_TYPE_BF16 / IFF_TYPE_F16
+ACTIVATIONS = {"silu": 0, "gelu": 1}                                 # IFF_ACT_SILU / IFF_ACT_GELU
 
 
 # name -> (restype, argtypes); must list every function include/iffnerf_hip.h declares (tests/test_abi.py checks)
@@ -141,6 +143,14 @@ SIGNATURES = {
     "iff_topk_batched": (C.c_int, [_VP, _I32, _I64, _I32, _VP, _VP, _VP]),
     "iff_pose_from_topk_batched": (C.c_int, [_VP, _VP, _I32, _I32, _VP, _VP, _I64, _I64, c_float_p, _VP, _VP, _VP]),
     "iff_pose_errors": (C.c_int, [_VP, _VP, _VP, _I32, _I32, _VP, _VP]),
+    "iff_layer_norm_forward": (C.c_int, [_VP, _I32, _I64, _I64, _I64, _I64, _I32, _VP, _VP, _I32, _F, _VP, _VP, _VP]),
+    "iff_layer_norm_backward_workspace": (_SZ, [_I64, _I32]),
+    "iff_layer_norm_backward": (C.c_int, [_VP, _I32, _I64, _I64, _I64, _I64, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "iff_gated_mlp_forward_workspace": (_SZ, [_I32, _I64, _I32, _I32, _I32, _I32]),
+    "iff_gated_mlp_forward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "iff_gated_mlp_backward_workspace": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
+    "iff_gated_mlp_backward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "iff_dropout": (C.c_int, [_VP, _I32, _I64, _VP, _I32, _U64, _VP, _U64, _VP, _VP]),
 }
 
 

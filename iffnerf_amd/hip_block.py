@@ -1,0 +1,250 @@
+"""The feed-forward half of a transformer block with its gradients, on libiffnerf_hip: ``layer_norm``, ``gated_mlp``, ``dropout``.
+
+What fine-tuning the image backbone runs per block -- ``x + dropout(gated_mlp(layer_norm(x)))`` -- as differentiable functions of GPU
+tensors (the training loop of the reference, pose_estimation/train.py:97-119, back-propagates through the identification module and with
+it through pose_estimation/backbone.py:12-14).  ``hip_vit.train_natively`` installs them on a backbone module.  fp32, bf16 and fp16;
+arithmetic and sums are fp32, a result is rounded once; every gradient is the same bits on every run.  Calls run on the current stream of
+the tensors' device, allocate through torch (so they can be captured into a hipGraph; take the gradients of a captured step with
+``torch.autograd.grad``) and raise ``RuntimeError`` for what they do not serve, CPU tensors among it.  First derivatives only.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check, dptr, stream_ptr
+
+
+def _serves(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor (got {type(t).__name__})")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU (got device {t.device}); libiffnerf_hip has no CPU path")
+    if t.dtype not in _lib.TYPES:
+        raise RuntimeError(f"{name} must be fp32, bf16 or fp16 (got {t.dtype})")
+
+
+def _beside(t: torch.Tensor, x: torch.Tensor, name: str, shape, types) -> torch.Tensor:
+    """A parameter next to x: its device, one of ``types``, exactly ``shape``; contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor (got {type(t).__name__})")
+    if t.device != x.device:
+        raise RuntimeError(f"{name} is on {t.device}, the input on {x.device}")
+    if t.dtype not in types:
+        raise RuntimeError(f"{name} is {t.dtype}; with an input of {x.dtype} it must be one of {sorted(str(k) for k in types)}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    return t.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else dptr(t, t.dtype)
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+# ---------------------------------------------------------------------------------------------------- layer norm
+def _rows(x: torch.Tensor):
+    """x [..., D] as rows (i, j) at i s0 + j s1: (tensor, n0, n1, s0, s1).  A contiguous tensor, a slice of its second-last axis (the
+    patch tokens behind a class token) and anything else with at most two row strides is read in place; the rest is copied."""
+    D = x.shape[-1]
+    if D == 1 or x.stride(-1) == 1:
+        dims = []                                              # (size, stride), outermost first, adjacent axes merged
+        for n, s in zip(x.shape[:-1], x.stride()[:-1]):
+            if n == 1:
+                continue
+            if dims and dims[-1][1] == n * s:
+                dims[-1] = (dims[-1][0] * n, s)
+            else:
+                dims.append((n, s))
+        if len(dims) <= 2:
+            (n0, s0), (n1, s1) = ([(1, 0)] * (2 - len(dims)) + dims) if x.numel() else ((0, 0), (0, 0))
+            return x, n0, n1, s0, s1
+    return x.contiguous(), 1, x.numel() // D, 0, D
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _layer_norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_type = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        xr, n0, n1, s0, s1 = _rows(x)
+        D, dy = x.shape[-1], dy.contiguous()
+        par = weight.dtype if weight is not None else ctx.bias_type if ctx.bias_type is not None else x.dtype
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty(D, dtype=par, device=x.device) if need_w else None
+        db = torch.empty(D, dtype=par, device=x.device) if need_b else None
+        L = _lib.lib()
+        ws = _workspace(L.iff_layer_norm_backward_workspace(n0 * n1, D), x.device) if need_w or need_b else None
+        with torch.cuda.device(x.device):
+            check(L.iff_layer_norm_backward(xr.data_ptr(), _lib.TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _lib.TYPES[par], _ptr(stats),
+                                            _ptr(dy), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(),
+                                            stream_ptr(x.device)), "iff_layer_norm_backward")
+        return dx, dw, db, None
+
+
+def _layer_norm(x, weight, bias, eps, keep):
+    xr, n0, n1, s0, s1 = _rows(x)
+    D = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(n0 * n1, 2, dtype=torch.float32, device=x.device) if keep else None
+    par = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    with torch.cuda.device(x.device):
+        check(_lib.lib().iff_layer_norm_forward(xr.data_ptr(), _lib.TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _ptr(bias), _lib.TYPES[par],
+                                                eps, _ptr(y), _ptr(stats), stream_ptr(x.device)), "iff_layer_norm_forward")
+    return y, stats
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """Layer norm over the last axis of ``x`` [..., D] (any D >= 1): ``(x - mean) / sqrt(var + eps) * weight + bias``, in x's type and
+    shape, contiguous.  ``weight`` / ``bias`` [D]: fp32 or x's type, both the same.  Differentiable in all three.  Rows are read in place
+    where at most two strides describe them (``tokens[:, 1:]``); other layouts are copied first.  The default ``eps`` is the backbone's."""
+    _serves(x, "layer_norm: x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"layer_norm: x must have a last axis of at least one value (got shape {tuple(x.shape)})")
+    if not eps >= 0.0:
+        raise RuntimeError(f"layer_norm: eps must not be negative (got {eps})")
+    if weight is not None:
+        weight = _beside(weight, x, "layer_norm: weight", x.shape[-1:], {torch.float32, x.dtype})
+    if bias is not None:
+        bias = _beside(bias, x, "layer_norm: bias", x.shape[-1:], {torch.float32, x.dtype} if weight is None else {weight.dtype})
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _layer_norm(x, weight, bias, float(eps), False)[0]
+
+
+# ---------------------------------------------------------------------------------------------------- gated feed-forward
+def _mlp_forward(x, w12, b12, w3, b3, act, keep):
+    M, D = x.shape
+    H, O = w3.shape[1], w3.shape[0]
+    ty = _lib.TYPES[x.dtype]
+    y = torch.empty(M, O, dtype=x.dtype, device=x.device)
+    h = torch.empty(M, H, dtype=x.dtype, device=x.device) if keep else None
+    pq = torch.empty(2, M, H, dtype=torch.float32, device=x.device) if keep else None
+    L = _lib.lib()
+    need = int(L.iff_gated_mlp_forward_workspace(ty, M, D, H, O, int(keep)))
+    ws = _workspace(need, x.device) if need else None
+    with torch.cuda.device(x.device):
+        check(L.iff_gated_mlp_forward(_ptr(x), ty, M, D, H, O, _ptr(w12), _ptr(b12), _ptr(w3), _ptr(b3), act, _ptr(y), _ptr(h), _ptr(pq), _ptr(ws),
+                                      0 if ws is None else ws.numel(), stream_ptr(x.device)), "iff_gated_mlp_forward")
+    return y, h, pq
+
+
+class _GatedMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w12, b12, w3, b3, act):
+        y, h, pq = _mlp_forward(x, w12, b12, w3, b3, act, True)
+        ctx.save_for_backward(x, w12, w3, h, pq)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w12, w3, h, pq = ctx.saved_tensors
+        M, D = x.shape
+        H, O = w3.shape[1], w3.shape[0]
+        ty, dy = _lib.TYPES[x.dtype], dy.contiguous()
+        need = ctx.needs_input_grad
+
+        def out(i, *shape):
+            return torch.empty(*shape, dtype=x.dtype, device=x.device) if need[i] else None
+
+        dx, dw12, db12, dw3, db3 = out(0, M, D), out(1, 2 * H, D), out(2, 2 * H), out(3, O, H), out(4, O)
+        L = _lib.lib()
+        ws = _workspace(L.iff_gated_mlp_backward_workspace(ty, M, D, H, O), x.device)
+        with torch.cuda.device(x.device):
+            check(L.iff_gated_mlp_backward(_ptr(x), ty, M, D, H, O, _ptr(w12), _ptr(w3), _ptr(h), _ptr(pq), _ptr(dy), _ptr(dx), _ptr(dw12),
+                                           _ptr(db12), _ptr(dw3), _ptr(db3), _ptr(ws), ws.numel(), stream_ptr(x.device)),
+                  "iff_gated_mlp_backward")
+        return dx, dw12, db12, dw3, db3, None
+
+
+def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w3: torch.Tensor, b3: Optional[torch.Tensor],
+              activation: str = "silu") -> torch.Tensor:
+    """Gated feed-forward block: ``[g | u] = x @ w12.T + b12``, ``(act(g) * u) @ w3.T + b3``.  ``x`` [..., D], ``w12`` [2 H, D] (gate rows
+    first -- the ``w12`` / ``w3`` layout of DINOv2's gated feed-forward), ``w3`` [O, H], biases [2 H] / [O] or None; one type and device.
+    ``activation``: "silu" or "gelu" (exact).  Differentiable in all five.  The hidden activation is rounded to the type once; what the
+    backward pass keeps next to it is fp32.  fp32 operands are multiplied as three bf16 pieces each, in fp32's accuracy; an infinite
+    fp32 operand gives NaN."""
+    _serves(x, "gated_mlp: x")
+    if activation not in _lib.ACTIVATIONS:
+        raise RuntimeError(f"gated_mlp: activation must be one of {sorted(_lib.ACTIVATIONS)} (got {activation!r})")
+    if x.dim() < 1 or not isinstance(w3, torch.Tensor) or w3.dim() != 2 or x.shape[-1] < 1 or min(w3.shape) < 1:
+        raise RuntimeError("gated_mlp: x [..., D], w12 [2 H, D], w3 [O, H] with no empty width expected")
+    D, (O, H) = x.shape[-1], w3.shape
+    w12 = _beside(w12, x, "gated_mlp: w12", (2 * H, D), {x.dtype})
+    w3 = _beside(w3, x, "gated_mlp: w3", (O, H), {x.dtype})
+    b12 = None if b12 is None else _beside(b12, x, "gated_mlp: b12", (2 * H,), {x.dtype})
+    b3 = None if b3 is None else _beside(b3, x, "gated_mlp: b3", (O,), {x.dtype})
+    x2 = x.reshape(-1, D).contiguous()
+    act = _lib.ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w12, b12, w3, b3)):
+        y = _GatedMlp.apply(x2, w12, b12, w3, b3, act)
+    else:
+        y = _mlp_forward(x2, w12, b12, w3, b3, act, False)[0]
+    return y.reshape(*x.shape[:-1], O)
+
+
+# ---------------------------------------------------------------------------------------------------- dropout
+def _dropout(x, residual, threshold, seed, seed_dev, offset):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        check(_lib.lib().iff_dropout(_ptr(x), _lib.TYPES[x.dtype], x.numel(), _ptr(residual), threshold, seed,
+                                     None if seed_dev is None else dptr(seed_dev, torch.int64, "seed"), offset, _ptr(y), stream_ptr(x.device)),
+              "iff_dropout")
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, threshold, seed, seed_dev, offset):
+        ctx.save_for_backward(seed_dev)           # (a seed tensor that changes before the backward pass is noticed by its version)
+        ctx.how = (threshold, seed, offset)
+        return _dropout(x, residual, threshold, seed, seed_dev, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        threshold, seed, offset = ctx.how
+        dx = _dropout(dy.contiguous(), None, threshold, seed, ctx.saved_tensors[0], offset) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: int = 0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``residual + x * keep / (1 - p)`` without a stored mask: ``keep`` is a function of (seed, offset, index) -- 16 bits of Philox 4x32-10
+    per value, so ``p`` is taken to the nearest 2^-16 -- and the backward pass computes it again.  ``seed``: 0 <= int < 2^64, or an int64
+    tensor of one value on x's device, read when the kernel runs (a captured step draws a new one per replay by refilling it);
+    ``offset``: 0 <= int < 2^64, another stream of the same seed.  Two calls with equal (seed, offset) drop the same positions.  A dropped
+    value never reaches the result, not even as a NaN.  ``residual``: x's shape, type and device."""
+    _serves(x, "dropout: x")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"dropout: p must be between 0 and 1 (got {p})")
+    seed_dev = None
+    if isinstance(seed, torch.Tensor):
+        if seed.device != x.device or seed.dtype != torch.int64 or seed.numel() != 1:
+            raise RuntimeError(f"dropout: a seed tensor must be one int64 on {x.device} (got {tuple(seed.shape)} {seed.dtype} on {seed.device})")
+        seed_dev, seed = seed.contiguous(), 0
+    for name, v in (("seed", seed), ("offset", offset)):
+        if not isinstance(v, int) or not 0 <= v < 2 ** 64:
+            raise RuntimeError(f"dropout: {name} must be an integer of 0 .. 2^64 - 1 (got {v!r})")
+    if residual is not None:
+        residual = _beside(residual, x, "dropout: residual", x.shape, {x.dtype})
+    threshold = int(math.floor(p * 65536 + 0.5))
+    x = x.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, threshold, seed, seed_dev, offset)
+    return _dropout(x, residual, threshold, seed, seed_dev, offset)

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define IFF_ABI_VERSION 12
+#define IFF_ABI_VERSION 13
 
 #define IFF_ERR_INVALID_ARGUMENT 1001
 #define IFF_ERR_UNSUPPORTED      1002
@@ -539,6 +539,54 @@ int iff_pose_from_topk_batched(const int64_t* idx, const float* val, int32_t Q, 
  * kept -- NaN when parts_opt is NULL --, translation error || gt[:3,3] - c2w[:3,3] ||, angular error in degrees
  * rad2deg(acos(clamp((trace(R_gt R^-1) - 1) / 2, -1, 1))) with the inverse by pivoted LU as torch.linalg.inv, rays kept). */
 int iff_pose_errors(const float* c2w, const float* gt_c2w, const float* parts_opt, int32_t Q, int32_t k, float* summary, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ trainable block operators
+ * The feed-forward half of a pre-norm transformer block, x + dropout(gated_mlp(layer_norm(x))), WITH its gradients: what fine-tuning the
+ * image backbone (pose_estimation/backbone.py:12-14) inside pose_estimation/train.py:97-119 runs per block.  Tensors are fp32, bf16 or
+ * fp16 (IFF_TYPE_*), arithmetic and every sum fp32; results are rounded to the tensors' type once.  Row counts are below 2^31, widths
+ * below 2^30; empty tensors are no-ops (gradients of parameters over no rows are zero).  Calls are reproducible bit for bit: no atomics. */
+#define IFF_TYPE_F32  0
+#define IFF_TYPE_BF16 1
+#define IFF_TYPE_F16  2
+#define IFF_ACT_SILU  0              /* g / (1 + exp(-g)) */
+#define IFF_ACT_GELU  1              /* g (1 + erf(g / sqrt 2)) / 2 */
+
+/* Layer norm over the last axis (the norms of the backbone's blocks, pose_estimation/backbone.py:12-14):
+ *   y = (x - mean) / sqrt(var + eps) * w + b,  mean and (biased) var over the row's `width` values.
+ * Row (i, j) of x, i < n0, j < n1, starts at i * stride0 + j * stride1 elements (a contiguous tensor, or the patch tokens behind the class
+ * token of [n0, 1 + n1, width]); y is contiguous [n0 * n1, width].  w_opt / b_opt [width] of type par_type (IFF_TYPE_F32 or x_type).
+ * stats_opt [n0 * n1, 2] = (mean, 1 / sqrt(var + eps)), fp32: what the backward pass reads. */
+int iff_layer_norm_forward(const void* x, int32_t x_type, int64_t n0, int64_t n1, int64_t stride0, int64_t stride1, int32_t width,
+                           const void* w_opt, const void* b_opt, int32_t par_type, float eps, void* y, float* stats_opt, void* stream);
+size_t iff_layer_norm_backward_workspace(int64_t rows, int32_t width);
+/* Gradients of the call above (autograd's backward in pose_estimation/train.py:119): dy contiguous [rows, width] -> dx_opt contiguous in
+ * x_type, dw_opt / db_opt [width] in par_type (sums over the rows in a fixed order).  Workspace: only where dw_opt or db_opt is given. */
+int iff_layer_norm_backward(const void* x, int32_t x_type, int64_t n0, int64_t n1, int64_t stride0, int64_t stride1, int32_t width,
+                            const void* w_opt, int32_t par_type, const float* stats, const void* dy, void* dx_opt, void* dw_opt, void* db_opt,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated feed-forward block (the MLP half of a backbone block, pose_estimation/backbone.py:12-14, in its gated form):
+ *   [g | u] = x w12^T + b12,  h = act(g) u,  y = h w3^T + b3
+ * x [M, D], w12 [2H, D] (gate rows first), w3 [O, H], b12_opt [2H], b3_opt [O], y [M, O]: one type, contiguous.  For the backward pass
+ * h_opt [M, H] (same type) and factors_opt [2, M, H] fp32 = (u act'(g), act(g)) are kept -- both or neither.  Workspace:
+ * iff_gated_mlp_forward_workspace (0 where h_opt is given may still be passed). */
+size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, int32_t keeps_h);
+int iff_gated_mlp_forward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12, const void* b12_opt,
+                          const void* w3, const void* b3_opt, int32_t activation, void* y, void* h_opt, float* factors_opt, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* Its gradients (autograd's backward in pose_estimation/train.py:119): dy [M, O] -> the outputs that are not NULL, in the operands' type. */
+size_t iff_gated_mlp_backward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
+int iff_gated_mlp_backward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12, const void* w3,
+                           const void* h, const float* factors, const void* dy, void* dx_opt, void* dw12_opt, void* db12_opt, void* dw3_opt,
+                           void* db3_opt, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Dropout without a stored mask (the dropout of a backbone block under pose_estimation/train.py:97-119):
+ *   y[i] = residual_opt[i] + (keep_i ? x[i] / (1 - p) : 0),  p = threshold / 65536
+ * keep_i: the 16 bits of value i are >= threshold (0 .. 65536).  The bits are those of Philox 4x32 with 10 rounds at counter
+ * (i / 8, offset) and key `seed` (or *seed_dev_opt, read on the device): bits 16 (i % 2) .. of word (i % 8) / 2.  The backward pass is
+ * the same call on dy without a residual.  A dropped value is not multiplied: an infinity or NaN there does not reach y. */
+int iff_dropout(const void* x, int32_t type, int64_t n, const void* residual_opt, int32_t threshold, uint64_t seed,
+                const uint64_t* seed_dev_opt, uint64_t offset, void* y, void* stream);
 
 #ifdef __cplusplus
 }
