@@ -20,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libiffnerf_hip.so")
 SOURCES = ["api.hip", "field_kernels.hip", "march_kernels.hip", "fan_march_kernels.hip", "fan8_march_kernels.hip", "march_grad_kernels.hip", "sampler_kernels.hip", "identify_kernels.hip", "trunk_f16_kernels.hip", "vit_kernels.hip",
-           "pose_kernels.hip", "shard_kernels.hip", "block_kernels.hip", "ffn_kernels.hip"]
+           "pose_kernels.hip", "shard_kernels.hip", "block/block_api.hip", "block/block_kernels.hip", "block/ffn_kernels.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
@@ -37,13 +37,13 @@ def _newer(target: str, deps) -> bool:
 def build(verbose: bool = False, force: bool = False, extra_flags=(), tag: str = "") -> str:
     """``tag``: a development variant -- objects under build/<tag>/, library build/lib_<tag>.so (load it with IFF_LIB_PATH); the
     in-tree product library is left alone."""
-    headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
+    headers = [os.path.join(d, h) for d in (CSRC, os.path.join(CSRC, "block")) for h in os.listdir(d) if h.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "iffnerf_hip.h"))
     objdir, lib = CSRC, LIB
     if tag:
         objdir = os.path.join(os.path.dirname(HERE), "build", tag)
         lib = os.path.join(os.path.dirname(HERE), "build", f"lib_{tag}.so")
-        os.makedirs(objdir, exist_ok=True)
+        os.makedirs(os.path.join(objdir, "block"), exist_ok=True)
     objs, jobs = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

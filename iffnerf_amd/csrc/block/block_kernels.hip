@@ -6,7 +6,7 @@
 //     e = dy w,   dx = r (e - mean(e) - xh mean(e xh)),   dw = sum_rows dy xh,   db = sum_rows dy
 // A row is read once into registers (the variance is the second pass over the REGISTERS: no cancellation of E[x^2] - mean^2), so the
 // forward pass moves x and y and nothing else; the backward pass moves x, dy and dx.  Both are bound by memory.
-#include "iff_launch.h"
+#include "block_launch.h"
 #include "block_types.h"
 
 #include <algorithm>

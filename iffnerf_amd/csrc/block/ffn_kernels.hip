@@ -7,7 +7,7 @@
 // hidden unit sit in the same lane's accumulators), and so are dh and the two factors' products.
 // The forward pass keeps h in the activations' type (it is the second product's operand) and p, q in fp32: rounding them too would
 // add a third rounding between dy and dx (measured against 64 bits: 2.1 roundings' worth instead of 1.4).
-#include "iff_launch.h"
+#include "block_launch.h"
 #include "block_types.h"
 
 #include <algorithm>

@@ -16,7 +16,34 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, dptr, stream_ptr
+from ._lib import check
+
+
+# A small call is bound by the host: what a backward pass runs on autograd's own thread costs three times what it costs in a loop
+# (forward + backward of a 8 x 64 dropout: 108 us with the guards of the other wrappers, 60-70 us with these, 55 us for torch's own product).
+_TYPES = _lib.TYPES
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _run(name: str, device: torch.device, *args) -> None:
+    """Entry point ``name`` with ``args`` on the current stream of ``device``."""
+    i, fn = device.index, getattr(_lib._lib or _lib.lib(), name)
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        check(rc, name)
+
+
+def _first_derivative(backward):
+    """``once_differentiable``, entered only where a second derivative could be asked for (autograd runs backward in grad mode then)."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, dy):
+        return guarded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+    return run
 
 
 def _serves(t: torch.Tensor, name: str) -> None:
@@ -24,29 +51,29 @@ def _serves(t: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} must be a tensor (got {type(t).__name__})")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on the GPU (got device {t.device}); libiffnerf_hip has no CPU path")
-    if t.dtype not in _lib.TYPES:
+    if t.dtype not in _TYPES:
         raise RuntimeError(f"{name} must be fp32, bf16 or fp16 (got {t.dtype})")
 
 
-def _beside(t: torch.Tensor, x: torch.Tensor, name: str, shape, types) -> torch.Tensor:
+def _beside(t: torch.Tensor, x: torch.Tensor, name: str, shape, *types) -> torch.Tensor:
     """A parameter next to x: its device, one of ``types``, exactly ``shape``; contiguous."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor (got {type(t).__name__})")
     if t.device != x.device:
         raise RuntimeError(f"{name} is on {t.device}, the input on {x.device}")
     if t.dtype not in types:
-        raise RuntimeError(f"{name} is {t.dtype}; with an input of {x.dtype} it must be one of {sorted(str(k) for k in types)}")
-    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} is {t.dtype}; with an input of {x.dtype} it must be {' or '.join(str(k) for k in types)}")
+    if t.shape != shape:
         raise RuntimeError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
     return t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else dptr(t, t.dtype)
+    return None if t is None else t.data_ptr()
 
 
-def _workspace(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor:
+    return x.new_empty((max(nbytes, 16),), dtype=torch.uint8)
 
 
 # ---------------------------------------------------------------------------------------------------- layer norm
@@ -54,6 +81,8 @@ def _rows(x: torch.Tensor):
     """x [..., D] as rows (i, j) at i s0 + j s1: (tensor, n0, n1, s0, s1).  A contiguous tensor, a slice of its second-last axis (the
     patch tokens behind a class token) and anything else with at most two row strides is read in place; the rest is copied."""
     D = x.shape[-1]
+    if x.is_contiguous():
+        return x, 1, x.numel() // D, 0, D
     if D == 1 or x.stride(-1) == 1:
         dims = []                                              # (size, stride), outermost first, adjacent axes merged
         for n, s in zip(x.shape[:-1], x.stride()[:-1]):
@@ -78,34 +107,32 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         xr, n0, n1, s0, s1 = _rows(x)
         D, dy = x.shape[-1], dy.contiguous()
         par = weight.dtype if weight is not None else ctx.bias_type if ctx.bias_type is not None else x.dtype
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(D, dtype=par, device=x.device) if need_w else None
-        db = torch.empty(D, dtype=par, device=x.device) if need_b else None
-        L = _lib.lib()
-        ws = _workspace(L.iff_layer_norm_backward_workspace(n0 * n1, D), x.device) if need_w or need_b else None
-        with torch.cuda.device(x.device):
-            check(L.iff_layer_norm_backward(xr.data_ptr(), _lib.TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _lib.TYPES[par], _ptr(stats),
-                                            _ptr(dy), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(),
-                                            stream_ptr(x.device)), "iff_layer_norm_backward")
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        dw = x.new_empty((D,), dtype=par) if need_w else None
+        db = x.new_empty((D,), dtype=par) if need_b else None
+        nbytes, ws = 0, None
+        if need_w or need_b:
+            nbytes = _lib._lib.iff_layer_norm_backward_workspace(n0 * n1, D)
+            ws = _workspace(nbytes, x)
+        _run("iff_layer_norm_backward", x.device, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _TYPES[par],
+             stats.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, dw, db, None
 
 
 def _layer_norm(x, weight, bias, eps, keep):
     xr, n0, n1, s0, s1 = _rows(x)
-    D = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(n0 * n1, 2, dtype=torch.float32, device=x.device) if keep else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = x.new_empty((n0 * n1, 2), dtype=torch.float32) if keep else None
     par = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    with torch.cuda.device(x.device):
-        check(_lib.lib().iff_layer_norm_forward(xr.data_ptr(), _lib.TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _ptr(bias), _lib.TYPES[par],
-                                                eps, _ptr(y), _ptr(stats), stream_ptr(x.device)), "iff_layer_norm_forward")
+    _run("iff_layer_norm_forward", x.device, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, x.shape[-1], _ptr(weight), _ptr(bias), _TYPES[par],
+         eps, y.data_ptr(), _ptr(stats))
     return y, stats
 
 
@@ -119,9 +146,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if not eps >= 0.0:
         raise RuntimeError(f"layer_norm: eps must not be negative (got {eps})")
     if weight is not None:
-        weight = _beside(weight, x, "layer_norm: weight", x.shape[-1:], {torch.float32, x.dtype})
+        weight = _beside(weight, x, "layer_norm: weight", x.shape[-1:], torch.float32, x.dtype)
     if bias is not None:
-        bias = _beside(bias, x, "layer_norm: bias", x.shape[-1:], {torch.float32, x.dtype} if weight is None else {weight.dtype})
+        bias = _beside(bias, x, "layer_norm: bias", x.shape[-1:], *((torch.float32, x.dtype) if weight is None else (weight.dtype,)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm(x, weight, bias, float(eps), False)[0]
@@ -130,17 +157,15 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 # ---------------------------------------------------------------------------------------------------- gated feed-forward
 def _mlp_forward(x, w12, b12, w3, b3, act, keep):
     M, D = x.shape
-    H, O = w3.shape[1], w3.shape[0]
-    ty = _lib.TYPES[x.dtype]
-    y = torch.empty(M, O, dtype=x.dtype, device=x.device)
-    h = torch.empty(M, H, dtype=x.dtype, device=x.device) if keep else None
-    pq = torch.empty(2, M, H, dtype=torch.float32, device=x.device) if keep else None
-    L = _lib.lib()
-    need = int(L.iff_gated_mlp_forward_workspace(ty, M, D, H, O, int(keep)))
-    ws = _workspace(need, x.device) if need else None
-    with torch.cuda.device(x.device):
-        check(L.iff_gated_mlp_forward(_ptr(x), ty, M, D, H, O, _ptr(w12), _ptr(b12), _ptr(w3), _ptr(b3), act, _ptr(y), _ptr(h), _ptr(pq), _ptr(ws),
-                                      0 if ws is None else ws.numel(), stream_ptr(x.device)), "iff_gated_mlp_forward")
+    O, H = w3.shape
+    ty = _TYPES[x.dtype]
+    y = x.new_empty((M, O))
+    h = x.new_empty((M, H)) if keep else None
+    pq = x.new_empty((2, M, H), dtype=torch.float32) if keep else None
+    nbytes = (_lib._lib or _lib.lib()).iff_gated_mlp_forward_workspace(ty, M, D, H, O, keep)
+    ws = _workspace(nbytes, x) if nbytes else None
+    _run("iff_gated_mlp_forward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), _ptr(b12), w3.data_ptr(), _ptr(b3), act, y.data_ptr(),
+         _ptr(h), _ptr(pq), _ptr(ws), nbytes)
     return y, h, pq
 
 
@@ -152,24 +177,22 @@ class _GatedMlp(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         x, w12, w3, h, pq = ctx.saved_tensors
         M, D = x.shape
-        H, O = w3.shape[1], w3.shape[0]
-        ty, dy = _lib.TYPES[x.dtype], dy.contiguous()
+        O, H = w3.shape
+        ty, dy = _TYPES[x.dtype], dy.contiguous()
         need = ctx.needs_input_grad
-
-        def out(i, *shape):
-            return torch.empty(*shape, dtype=x.dtype, device=x.device) if need[i] else None
-
-        dx, dw12, db12, dw3, db3 = out(0, M, D), out(1, 2 * H, D), out(2, 2 * H), out(3, O, H), out(4, O)
-        L = _lib.lib()
-        ws = _workspace(L.iff_gated_mlp_backward_workspace(ty, M, D, H, O), x.device)
-        with torch.cuda.device(x.device):
-            check(L.iff_gated_mlp_backward(_ptr(x), ty, M, D, H, O, _ptr(w12), _ptr(w3), _ptr(h), _ptr(pq), _ptr(dy), _ptr(dx), _ptr(dw12),
-                                           _ptr(db12), _ptr(dw3), _ptr(db3), _ptr(ws), ws.numel(), stream_ptr(x.device)),
-                  "iff_gated_mlp_backward")
+        dx = x.new_empty((M, D)) if need[0] else None
+        dw12 = x.new_empty((2 * H, D)) if need[1] else None
+        db12 = x.new_empty((2 * H,)) if need[2] else None
+        dw3 = x.new_empty((O, H)) if need[3] else None
+        db3 = x.new_empty((O,)) if need[4] else None
+        nbytes = _lib._lib.iff_gated_mlp_backward_workspace(ty, M, D, H, O)
+        ws = _workspace(nbytes, x)
+        _run("iff_gated_mlp_backward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), h.data_ptr(), pq.data_ptr(),
+             dy.data_ptr(), _ptr(dx), _ptr(dw12), _ptr(db12), _ptr(dw3), _ptr(db3), ws.data_ptr(), ws.numel())
         return dx, dw12, db12, dw3, db3, None
 
 
@@ -186,10 +209,10 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
     if x.dim() < 1 or not isinstance(w3, torch.Tensor) or w3.dim() != 2 or x.shape[-1] < 1 or min(w3.shape) < 1:
         raise RuntimeError("gated_mlp: x [..., D], w12 [2 H, D], w3 [O, H] with no empty width expected")
     D, (O, H) = x.shape[-1], w3.shape
-    w12 = _beside(w12, x, "gated_mlp: w12", (2 * H, D), {x.dtype})
-    w3 = _beside(w3, x, "gated_mlp: w3", (O, H), {x.dtype})
-    b12 = None if b12 is None else _beside(b12, x, "gated_mlp: b12", (2 * H,), {x.dtype})
-    b3 = None if b3 is None else _beside(b3, x, "gated_mlp: b3", (O,), {x.dtype})
+    w12 = _beside(w12, x, "gated_mlp: w12", (2 * H, D), x.dtype)
+    w3 = _beside(w3, x, "gated_mlp: w3", (O, H), x.dtype)
+    b12 = None if b12 is None else _beside(b12, x, "gated_mlp: b12", (2 * H,), x.dtype)
+    b3 = None if b3 is None else _beside(b3, x, "gated_mlp: b3", (O,), x.dtype)
     x2 = x.reshape(-1, D).contiguous()
     act = _lib.ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w12, b12, w3, b3)):
@@ -201,11 +224,8 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
 
 # ---------------------------------------------------------------------------------------------------- dropout
 def _dropout(x, residual, threshold, seed, seed_dev, offset):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        check(_lib.lib().iff_dropout(_ptr(x), _lib.TYPES[x.dtype], x.numel(), _ptr(residual), threshold, seed,
-                                     None if seed_dev is None else dptr(seed_dev, torch.int64, "seed"), offset, _ptr(y), stream_ptr(x.device)),
-              "iff_dropout")
+    y = torch.empty_like(x)
+    _run("iff_dropout", x.device, x.data_ptr(), _TYPES[x.dtype], x.numel(), _ptr(residual), threshold, seed, _ptr(seed_dev), offset, y.data_ptr())
     return y
 
 
@@ -217,11 +237,12 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, residual, threshold, seed, seed_dev, offset)
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         threshold, seed, offset = ctx.how
-        dx = _dropout(dy.contiguous(), None, threshold, seed, ctx.saved_tensors[0], offset) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+        need = ctx.needs_input_grad
+        dx = _dropout(dy.contiguous(), None, threshold, seed, ctx.saved_tensors[0], offset) if need[0] else None
+        return dx, dy if need[1] else None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: int = 0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -242,7 +263,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
         if not isinstance(v, int) or not 0 <= v < 2 ** 64:
             raise RuntimeError(f"dropout: {name} must be an integer of 0 .. 2^64 - 1 (got {v!r})")
     if residual is not None:
-        residual = _beside(residual, x, "dropout: residual", x.shape, {x.dtype})
+        residual = _beside(residual, x, "dropout: residual", x.shape, x.dtype)
     threshold = int(math.floor(p * 65536 + 0.5))
     x = x.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):

@@ -7,6 +7,9 @@ reads) runs in libiffnerf_hip under ``torch.no_grad`` while the module -- class,
 reference's ``create_backbone`` returns; with autograd enabled on a trainable backbone the module's own torch forward runs.
 State-dict keys of both sources are understood (``blocks.i.attn.qkv.*``, ``blocks.i.ls1.gamma``, ``blocks.i.mlp.fc1.*`` for
 DINOv2; ``blocks.i.qkv.*``, ``blocks.i.ls1``, ``blocks.i.fc1.*`` for the stand-in).
+
+``train_natively`` is the counterpart for that torch forward: the layer norms, gated feed-forwards and dropouts inside a backbone run their
+forward AND backward passes on ``hip_block``'s operators.
 """
 from __future__ import annotations
 
@@ -17,7 +20,7 @@ from typing import Dict, Optional
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, hip_block
 from ._lib import check, dptr, stream_ptr
 
 
@@ -228,3 +231,87 @@ def restore_stock(module: torch.nn.Module) -> torch.nn.Module:
 
 def is_served_natively(module: torch.nn.Module) -> bool:
     return isinstance(module.__dict__.get("forward_features"), _NativeForwardFeatures)
+
+
+# ---------------------------------------------------------------------------------------------------- training
+def _autocast(*tensors):
+    """What an autocast region casts the operands of a matrix product to; outside one, the tensors as they are."""
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    dt = torch.get_autocast_dtype("cuda")
+    return tuple(t if t is None or not t.is_floating_point() else t.to(dt) for t in tensors)
+
+
+class _NativeForward:
+    """The callable installed as a sub-module's ``forward`` by ``train_natively``.  It reads the module's own parameters at every call:
+    optimizer steps, ``.to(...)`` and ``load_state_dict`` need nothing else."""
+
+    def __init__(self, module: torch.nn.Module):
+        self.module = module
+
+
+class _NativeLayerNorm(_NativeForward):
+    def __call__(self, x):
+        m = self.module
+        return hip_block.layer_norm(x, m.weight, m.bias, m.eps)
+
+
+class _NativeGatedMlp(_NativeForward):
+    def __call__(self, x):
+        m = self.module
+        return hip_block.gated_mlp(*_autocast(x, m.w12.weight, m.w12.bias, m.w3.weight, m.w3.bias))
+
+
+def _fresh_seed(x: torch.Tensor) -> torch.Tensor:
+    # one value of torch's own generator on the device: follows torch.manual_seed, is replayed by activation checkpointing, and a
+    # captured step draws another one at every replay
+    return torch.empty(1, dtype=torch.int64, device=x.device).random_()
+
+
+class _NativeDropout(_NativeForward):
+    def __call__(self, x):
+        m = self.module
+        return hip_block.dropout(x, m.p, _fresh_seed(x)) if m.training and m.p > 0.0 else x
+
+
+class _NativeDropAdd(_NativeForward):
+    def __call__(self, residual, branch):
+        m = self.module
+        if not (m.training and m.p > 0.0):
+            return residual + branch
+        return hip_block.dropout(branch.to(residual.dtype), m.p, _fresh_seed(branch), residual=residual)
+
+
+def _native_forward(m: torch.nn.Module):
+    from .pose_estimation.backbone import _DropAdd
+    if isinstance(m, torch.nn.LayerNorm) and len(m.normalized_shape) == 1:
+        return _NativeLayerNorm(m)
+    if isinstance(m, torch.nn.Dropout) and not m.inplace:
+        return _NativeDropout(m)
+    if isinstance(m, _DropAdd):
+        return _NativeDropAdd(m)
+    w12, w3 = getattr(m, "w12", None), getattr(m, "w3", None)
+    if isinstance(w12, torch.nn.Linear) and isinstance(w3, torch.nn.Linear) and w12.out_features == 2 * w3.in_features:
+        return _NativeGatedMlp(m)
+    return None
+
+
+def train_natively(module: torch.nn.Module) -> torch.nn.Module:
+    """Run the layer norms, gated feed-forwards (``w12`` / ``w3`` as in DINOv2, SiLU) and dropouts inside ``module`` -- a backbone that
+    pose_estimation/train.py:97-119 back-propagates through -- on ``hip_block``'s operators, forward and backward, and return THE SAME
+    module.  As with ``serve_natively`` nothing is wrapped: classes, parameters and ``state_dict`` keys stay, one instance attribute
+    ``forward`` per sub-module is installed.  The module then needs GPU tensors; values differ from stock torch by rounding, and a dropout's
+    mask comes from another generator (seeded by torch's).  ``train_stock(module)`` removes it; without this call nothing changes."""
+    for m in module.modules():
+        f = _native_forward(m)
+        if f is not None:
+            object.__setattr__(m, "forward", f)
+    return module
+
+
+def train_stock(module: torch.nn.Module) -> torch.nn.Module:
+    """Undo ``train_natively``: every sub-module's ``forward`` is its class's method again."""
+    for m in module.modules():
+        if isinstance(m.__dict__.get("forward"), _NativeForward):
+            object.__delattr__(m, "forward")
+    return module

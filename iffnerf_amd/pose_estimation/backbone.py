@@ -60,15 +60,41 @@ class _Mlp(torch.nn.Module):
         return self.fc2(F.gelu(self.fc1(x)))
 
 
-class _Block(torch.nn.Module):
-    def __init__(self, dim, heads, mlp):
+class _GatedMlp(torch.nn.Module):
+    """DINOv2's gated feed-forward: ``w12`` holds the gate rows, then the up rows; the hidden width keeps the ungated block's parameters
+    (two thirds of ``hidden``, up to a multiple of 8)."""
+
+    def __init__(self, dim, hidden):
         super().__init__()
-        self.norm1, self.attn, self.ls1 = torch.nn.LayerNorm(dim, eps=1e-6), _Attention(dim, heads), _LayerScale(dim)
-        self.norm2, self.mlp, self.ls2 = torch.nn.LayerNorm(dim, eps=1e-6), _Mlp(dim, mlp), _LayerScale(dim)
+        hidden = (int(hidden * 2 / 3) + 7) // 8 * 8
+        self.w12, self.w3 = torch.nn.Linear(dim, 2 * hidden), torch.nn.Linear(hidden, dim)
 
     def forward(self, x):
-        x = x + self.ls1(self.attn(self.norm1(x)))
-        return x + self.ls2(self.mlp(self.norm2(x)))
+        gate, up = self.w12(x).chunk(2, dim=-1)
+        return self.w3(F.silu(gate) * up)
+
+
+class _DropAdd(torch.nn.Module):
+    """``residual + dropout(branch)``; with p = 0 or in evaluation the plain sum."""
+
+    def __init__(self, p):
+        super().__init__()
+        self.p = p
+
+    def forward(self, residual, branch):
+        return residual + (F.dropout(branch, self.p, self.training) if self.p else branch)
+
+
+class _Block(torch.nn.Module):
+    def __init__(self, dim, heads, mlp, ffn="mlp", drop=0.0):
+        super().__init__()
+        self.norm1, self.attn, self.ls1 = torch.nn.LayerNorm(dim, eps=1e-6), _Attention(dim, heads), _LayerScale(dim)
+        self.norm2, self.mlp, self.ls2 = torch.nn.LayerNorm(dim, eps=1e-6), {"mlp": _Mlp, "swiglu": _GatedMlp}[ffn](dim, mlp), _LayerScale(dim)
+        self.add1, self.add2 = _DropAdd(drop), _DropAdd(drop)
+
+    def forward(self, x):
+        x = self.add1(x, self.ls1(self.attn(self.norm1(x))))
+        return self.add2(x, self.ls2(self.mlp(self.norm2(x))))
 
 
 class _PatchEmbed(torch.nn.Module):
@@ -85,17 +111,21 @@ class SeededViTS14(torch.nn.Module):
     ``pos_embed`` [1, 1 + 37 x 37, 384] (the 518-pixel pretraining grid, resized bicubically to the input's grid as DINOv2's
     ``interpolate_pos_encoding`` does), ``mask_token``, ``patch_embed.proj``, 12 x ``blocks.i.{norm1, attn.qkv, attn.proj, ls1.gamma,
     norm2, mlp.fc1, mlp.fc2, ls2.gamma}``, ``norm``.  Randomly initialised from ``seed``: a stand-in for timing, plumbing and the
-    checkpoint-key contract, not a feature extractor."""
+    checkpoint-key contract, not a feature extractor.  ``ffn="swiglu"``: DINOv2's gated feed-forward (``mlp.w12``, ``mlp.w3``) in place of
+    ``fc1`` / ``fc2``; ``drop``: dropout on both branches of every block in training (no parameters, no keys)."""
 
-    def __init__(self, seed: int = 0, dim: int = 384, depth: int = 12, heads: int = 6, patch: int = 14, pretrain_grid: int = 37):
+    def __init__(self, seed: int = 0, dim: int = 384, depth: int = 12, heads: int = 6, patch: int = 14, pretrain_grid: int = 37,
+                 ffn: str = "mlp", drop: float = 0.0):
         super().__init__()
+        if ffn not in ("mlp", "swiglu") or not 0.0 <= drop < 1.0:
+            raise RuntimeError(f"ffn must be 'mlp' or 'swiglu' and drop in [0, 1) (got {ffn!r}, {drop})")
         gen = torch.Generator().manual_seed(seed)
         self.patch_size = patch
         self.cls_token = torch.nn.Parameter(torch.zeros(1, 1, dim))
         self.pos_embed = torch.nn.Parameter(torch.zeros(1, 1 + pretrain_grid * pretrain_grid, dim))
         self.mask_token = torch.nn.Parameter(torch.zeros(1, dim))
         self.patch_embed = _PatchEmbed(dim, patch)
-        self.blocks = torch.nn.ModuleList(_Block(dim, heads, 4 * dim) for _ in range(depth))
+        self.blocks = torch.nn.ModuleList(_Block(dim, heads, 4 * dim, ffn, drop) for _ in range(depth))
         self.norm = torch.nn.LayerNorm(dim, eps=1e-6)
         self.head = torch.nn.Identity()
         with torch.no_grad():

@@ -487,6 +487,93 @@ def test_first_derivatives_only(dev):
         g.sum().backward()
 
 
+# ------------------------------------------------------------------------------------------------------------ the backbone in training
+def backbone(ffn, drop, **kw):
+    from iffnerf_amd.pose_estimation.backbone import SeededViTS14
+    return SeededViTS14(seed=3, dim=96, depth=2, heads=3, pretrain_grid=4, ffn=ffn, drop=drop, **kw)
+
+
+def test_train_natively_keeps_the_module():
+    """Same object, keys and classes; undone without a trace; a copy serves its own parameters.  The default stand-in is untouched by the
+    gated form: the keys and values it always had."""
+    import copy
+    from iffnerf_amd import hip_vit
+    m = backbone("swiglu", 0.1)
+    keys, kinds = list(m.state_dict()), [type(k) for k in m.modules()]
+    assert "blocks.0.mlp.w12.weight" in keys and m.state_dict()["blocks.0.mlp.w12.weight"].shape == (512, 96)
+    assert hip_vit.train_natively(m) is m and list(m.state_dict()) == keys and [type(k) for k in m.modules()] == kinds
+    assert "forward" in m.norm.__dict__ and "forward" in m.blocks[1].mlp.__dict__ and "forward" not in m.blocks[1].attn.__dict__
+    c = copy.deepcopy(m)
+    assert c.norm.__dict__["forward"].module is c.norm
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        m.norm(torch.zeros(2, 96))
+    hip_vit.train_stock(m)
+    assert not any("forward" in k.__dict__ for k in m.modules())
+    m.norm(torch.zeros(2, 96))
+    plain = backbone("mlp", 0.0)
+    assert "blocks.0.mlp.fc1.weight" in plain.state_dict() and not any("add" in k for k in plain.state_dict())
+    for bad in (dict(ffn="relu", drop=0.0), dict(ffn="mlp", drop=1.0)):
+        with pytest.raises(RuntimeError, match="ffn must be"):
+            backbone(**bad)
+
+
+@gpu
+@pytest.mark.parametrize("ffn", ["mlp", "swiglu"])
+def test_a_backbone_trains_on_them(dev, ffn, monkeypatch):
+    """Gradients of every parameter against the same backbone in 64 bits, dropout off; with dropout on: the same seed gives the same step,
+    another seed another one, evaluation none.  Normwise 2^-15 relative: fp32 throughout, O(30) roundings of tensors and stock products
+    over up to 256 terms on the way, each well under 2^-21 of its norm."""
+    from iffnerf_amd import hip_vit
+    m = backbone(ffn, 0.0).to(dev)
+    img = normal((2, 3, 56, 56), 300)
+    want = backbone(ffn, 0.0).to(dev)
+    want.load_state_dict(m.state_dict())                                    # (the stand-in's biases are torch's own default)
+    want.double()
+    monkeypatch.setattr(hip_vit, "interpolate_pos_embed", lambda pos, *a, **k: pos[0])      # (the grid is the table's, and fp64 stays fp64)
+
+    def loss(net, x):
+        out = net.forward_features(x)["x_norm_patchtokens"]
+        return (out * torch.linspace(-1, 1, out.numel(), device=dev, dtype=out.dtype).view_as(out)).sum()
+
+    hip_vit.train_natively(m).train()
+    names = [n for n, p in m.named_parameters() if n not in ("mask_token",)]
+    got = torch.autograd.grad(loss(m, img), [dict(m.named_parameters())[n] for n in names])
+    ref = torch.autograd.grad(loss(want, img.double()), [dict(want.named_parameters())[n] for n in names])
+    for n, a, b in zip(names, got, ref):
+        assert float((a.double() - b).norm()) <= 2.0 ** -15 * float(b.norm()) + 1e-9, n
+    d = hip_vit.train_natively(backbone(ffn, 0.2).to(dev)).train()
+    d.load_state_dict(m.state_dict())
+
+    def step(seed):
+        torch.manual_seed(seed)
+        return torch.autograd.grad(loss(d, img), [d.blocks[0].norm1.weight])[0]
+
+    a, b, c = step(1), step(1), step(2)
+    assert torch.equal(a, b) and not torch.equal(a, c)
+    with torch.no_grad():
+        assert torch.equal(d.eval().forward_features(img)["x_prenorm"], m.eval().forward_features(img)["x_prenorm"])
+
+
+@gpu
+def test_a_backbone_step_under_autocast_and_checkpointing(dev):
+    from torch.utils.checkpoint import checkpoint
+    from iffnerf_amd import hip_vit
+    m = hip_vit.train_natively(backbone("swiglu", 0.2).to(dev)).train()
+    x = normal((2, 17, 96), 301).requires_grad_(True)
+    torch.manual_seed(5)
+    plain = torch.autograd.grad(m.blocks[0](x).square().sum(), (x, m.blocks[0].mlp.w12.weight))
+    torch.manual_seed(5)
+    again = torch.autograd.grad(checkpoint(m.blocks[0], x, use_reentrant=False).square().sum(), (x, m.blocks[0].mlp.w12.weight))
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))             # the recomputation drops what the forward pass dropped
+    torch.manual_seed(5)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m.blocks[0](x)
+    assert y.dtype == torch.float32
+    g = torch.autograd.grad(y.square().sum(), (x, m.blocks[0].mlp.w12.weight))
+    for a, b in zip(g, plain):                                              # bf16 products: a dozen roundings of 2^-8
+        assert a.dtype == torch.float32 and float((a - b).norm() / b.norm()) <= 12 * 2.0 ** -8
+
+
 # ------------------------------------------------------------------------------------------------------------ refusals
 def test_cpu_tensors_are_refused():
     x, w = torch.zeros(2, 4), torch.zeros(4)
