@@ -146,10 +146,11 @@ SIGNATURES = {
     "iff_layer_norm_forward": (C.c_int, [_VP, _I32, _I64, _I64, _I64, _I64, _I32, _VP, _VP, _I32, _F, _VP, _VP, _VP]),
     "iff_layer_norm_backward_workspace": (_SZ, [_I64, _I32]),
     "iff_layer_norm_backward": (C.c_int, [_VP, _I32, _I64, _I64, _I64, _I64, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
-    "iff_gated_mlp_forward_workspace": (_SZ, [_I32, _I64, _I32, _I32, _I32, _I32]),
-    "iff_gated_mlp_forward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "iff_gated_mlp_kept_bytes": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
+    "iff_gated_mlp_forward_workspace": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
+    "iff_gated_mlp_forward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _VP, _VP, _SZ, _VP, _SZ, _VP]),
     "iff_gated_mlp_backward_workspace": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
-    "iff_gated_mlp_backward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "iff_gated_mlp_backward": (C.c_int, [_VP, _I32, _I64, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "iff_dropout": (C.c_int, [_VP, _I32, _I64, _VP, _I32, _U64, _VP, _U64, _VP, _VP]),
 }
 

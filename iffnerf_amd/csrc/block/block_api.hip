@@ -76,51 +76,61 @@ extern "C" int iff_layer_norm_backward(const void* x, int32_t x_type, int64_t n0
     return 0;
 }
 
+static int64_t ffn_limit() { return (int64_t)1 << 21; }          // 2 H and the operand rows of the tile kernel stay below 2^22
+
 static int check_ffn(const char* who, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
     IFF_REQUIRE(block_type(type), "%s: type %d is not one of IFF_TYPE_F32 / BF16 / F16", who, type);
     IFF_REQUIRE(M >= 0 && M <= INT32_MAX, "%s: bad row count %lld", who, (long long)M);
-    IFF_REQUIRE(D >= 1 && H >= 1 && O >= 1 && D <= block_limit() && H <= block_limit() / 2 && O <= block_limit(), "%s: bad widths D %d H %d O %d", who, D, H, O);
+    IFF_REQUIRE(D >= 1 && H >= 1 && O >= 1 && D <= ffn_limit() && H <= ffn_limit() / 2 && O <= ffn_limit(), "%s: bad widths D %d H %d O %d", who, D, H, O);
     return 0;
+}
+static bool ffn_ok(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
+    return block_type(type) && M > 0 && M <= INT32_MAX && D >= 1 && H >= 1 && O >= 1 && D <= ffn_limit() && H <= ffn_limit() / 2 && O <= ffn_limit();
 }
 static FfnArgs ffn_args(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
     FfnArgs a{};
     a.dt = type; a.M = M; a.D = D; a.H = H; a.O = O;
     return a;
 }
-extern "C" size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, int32_t keeps_h) {
-    if (!block_type(type) || M <= 0 || D < 1 || H < 1 || O < 1) return 0;
-    return ffn_forward_workspace(ffn_args(type, M, D, H, O), keeps_h != 0);
+extern "C" size_t iff_gated_mlp_kept_bytes(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
+    return ffn_ok(type, M, D, H, O) ? ffn_kept_bytes(ffn_args(type, M, D, H, O)) : 0;
+}
+extern "C" size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
+    return ffn_ok(type, M, D, H, O) ? ffn_forward_workspace(ffn_args(type, M, D, H, O)) : 0;
 }
 extern "C" int iff_gated_mlp_forward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12,
-                                     const void* b12_opt, const void* w3, const void* b3_opt, int32_t activation, void* y, void* h_opt,
-                                     float* factors_opt, void* workspace, size_t workspace_bytes, void* stream) {
+                                     const void* b12_opt, const void* w3, const void* b3_opt, int32_t activation, void* y, void* kept_opt,
+                                     size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_ffn("iff_gated_mlp_forward", type, M, D, H, O)) return rc;
     IFF_REQUIRE(activation == IFF_ACT_SILU || activation == IFF_ACT_GELU, "iff_gated_mlp_forward: activation %d is neither IFF_ACT_SILU nor IFF_ACT_GELU", activation);
     if (M == 0) return 0;
     IFF_REQUIRE(x && w12 && w3 && y, "iff_gated_mlp_forward: null buffer");
-    IFF_REQUIRE((h_opt != nullptr) == (factors_opt != nullptr), "iff_gated_mlp_forward: h and its factors are kept together or not at all");
-    const size_t need = iff_gated_mlp_forward_workspace(type, M, D, H, O, h_opt != nullptr);
-    if (need && (!workspace || workspace_bytes < need))
-        return fail(IFF_ERR_WORKSPACE, "iff_gated_mlp_forward: workspace %zu < %zu bytes", workspace_bytes, need);
     FfnArgs a = ffn_args(type, M, D, H, O);
-    a.act = activation; a.x = x; a.w12 = w12; a.b12 = b12_opt; a.w3 = w3; a.b3 = b3_opt; a.y = y; a.h = h_opt; a.pq = factors_opt;
+    if (kept_opt && kept_bytes < ffn_kept_bytes(a))
+        return fail(IFF_ERR_WORKSPACE, "iff_gated_mlp_forward: kept %zu < %zu bytes", kept_bytes, ffn_kept_bytes(a));
+    const size_t need = ffn_forward_workspace(a);
+    if (!workspace || workspace_bytes < need)
+        return fail(IFF_ERR_WORKSPACE, "iff_gated_mlp_forward: workspace %zu < %zu bytes", workspace_bytes, need);
+    IFF_REQUIRE((((uintptr_t)workspace | (uintptr_t)kept_opt) & 15) == 0, "iff_gated_mlp_forward: workspace and kept must be 16-byte aligned");
+    a.act = activation; a.x = x; a.w12 = w12; a.b12 = b12_opt; a.w3 = w3; a.b3 = b3_opt; a.y = y; a.kept = kept_opt;
     IFF_HIP(launch_ffn_forward(a, workspace, (hipStream_t)stream));
     return 0;
 }
 extern "C" size_t iff_gated_mlp_backward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O) {
-    if (!block_type(type) || M <= 0 || D < 1 || H < 1 || O < 1) return 0;
-    return ffn_backward_workspace(ffn_args(type, M, D, H, O));
+    if (M == 0) return ffn_ok(type, 1, D, H, O) ? ffn_backward_workspace(ffn_args(type, 0, D, H, O)) : 0;
+    return ffn_ok(type, M, D, H, O) ? ffn_backward_workspace(ffn_args(type, M, D, H, O)) : 0;
 }
 extern "C" int iff_gated_mlp_backward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12,
-                                      const void* w3, const void* h, const float* factors, const void* dy, void* dx_opt, void* dw12_opt,
-                                      void* db12_opt, void* dw3_opt, void* db3_opt, void* workspace, size_t workspace_bytes, void* stream) {
+                                      const void* w3, const void* kept, const void* dy, void* dx_opt, void* dw12_opt, void* db12_opt,
+                                      void* dw3_opt, void* db3_opt, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_ffn("iff_gated_mlp_backward", type, M, D, H, O)) return rc;
-    IFF_REQUIRE(M == 0 || (x && w12 && w3 && h && factors && dy), "iff_gated_mlp_backward: null buffer");
+    IFF_REQUIRE(M == 0 || (x && w12 && w3 && kept && dy), "iff_gated_mlp_backward: null buffer");
     const size_t need = iff_gated_mlp_backward_workspace(type, M, D, H, O);
-    if (need && (!workspace || workspace_bytes < need))
+    if (!workspace || workspace_bytes < need)
         return fail(IFF_ERR_WORKSPACE, "iff_gated_mlp_backward: workspace %zu < %zu bytes", workspace_bytes, need);
+    IFF_REQUIRE((((uintptr_t)workspace | (uintptr_t)kept) & 15) == 0, "iff_gated_mlp_backward: workspace and kept must be 16-byte aligned");
     FfnArgs a = ffn_args(type, M, D, H, O);
-    a.x = x; a.w12 = w12; a.w3 = w3; a.h = const_cast<void*>(h); a.pq = const_cast<float*>(factors); a.dy = dy;
+    a.x = x; a.w12 = w12; a.w3 = w3; a.kept = const_cast<void*>(kept); a.dy = dy;
     a.dx = dx_opt; a.dw12 = dw12_opt; a.db12 = db12_opt; a.dw3 = dw3_opt; a.db3 = db3_opt;
     IFF_HIP(launch_ffn_backward(a, workspace, (hipStream_t)stream));
     return 0;

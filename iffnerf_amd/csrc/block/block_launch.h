@@ -26,10 +26,11 @@ struct FfnArgs {
     int64_t M; int D, H, O;
     const void* x; const void* w12; const void* b12; const void* w3; const void* b3;
     void* y;
-    void* h; float* pq;                   // kept for the backward pass: h [M][H], p and q fp32 [2][M][H] (null when there is none)
+    void* kept;                           // what the backward pass reads (ffn_kept_bytes), null when there is none
     const void* dy; void* dx; void* dw12; void* db12; void* dw3; void* db3;
 };
-size_t ffn_forward_workspace(const FfnArgs& a, bool keeps_h);
+size_t ffn_kept_bytes(const FfnArgs& a);
+size_t ffn_forward_workspace(const FfnArgs& a);
 size_t ffn_backward_workspace(const FfnArgs& a);
 hipError_t launch_ffn_forward(const FfnArgs& a, void* ws, hipStream_t s);
 hipError_t launch_ffn_backward(const FfnArgs& a, void* ws, hipStream_t s);

@@ -3,10 +3,10 @@
 //     [g | u] = x W12^T + b12,   h = act(g) u,   y = h W3^T + b3                    x [M][D], W12 [2H][D], W3 [O][H]
 //     q = act(g), p = u act'(g):  dh = dy W3,  dg = dh p,  du = dh q
 //     dx = [dg | du] W12,  dW12 = [dg | du]^T x,  dW3 = dy^T h,  db12 = sum_m [dg | du],  db3 = sum_m dy
-// Six matrix products; both projections, the activation and the product of the first are ONE launch (the gate and up columns of a
-// hidden unit sit in the same lane's accumulators), and so are dh and the two factors' products.
-// The forward pass keeps h in the activations' type (it is the second product's operand) and p, q in fp32: rounding them too would
-// add a third rounding between dy and dx (measured against 64 bits: 2.1 roundings' worth instead of 1.4).
+// Six matrix products on one tile kernel; both projections, the activation and the product of the first are ONE launch (the gate and the
+// up column of a hidden unit sit in the same lane's accumulators), and so are dh and the products with its two factors.
+// The forward pass keeps h in the operand type (it is the second product's operand) and p, q in fp32: rounding them too would add a
+// third rounding between dy and dx (against 64 bits: 2.1 roundings' worth instead of 1.4).
 #include "block_launch.h"
 #include "block_types.h"
 
@@ -30,23 +30,22 @@ __device__ __forceinline__ void activation(int act, float g, float& f, float& df
     }
 }
 
-// matrix-core element of a type and its product; fp32 runs as three bf16 pieces a = a0 + a1 + a2 (8 bits each, by truncation: exact) and
-// the six products whose weight is above 2^-24
+// ------------------------------------------------------------------------------------------------ operands
+// The matrix cores' element of a type and the number of planes an operand of it has.  fp32 is multiplied as three bf16 planes
+// a = a0 + a1 + a2 (8 bits of the significand each, by truncation: exact) and the six plane products whose weight is above 2^-24.
 template <class T> struct Mat { typedef __bf16 e; static constexpr int P = 3; };
 template <> struct Mat<__bf16> { typedef __bf16 e; static constexpr int P = 1; };
 template <> struct Mat<_Float16> { typedef _Float16 e; static constexpr int P = 1; };
-typedef __bf16 vb8 __attribute__((ext_vector_type(8)));
-typedef _Float16 vh8 __attribute__((ext_vector_type(8)));
-template <class E> struct V8;
-template <> struct V8<__bf16> { typedef vb8 t; };
-template <> struct V8<_Float16> { typedef vh8 t; };
-__device__ __forceinline__ f32x16 mfma(vb8 a, vb8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mfma(vh8 a, vh8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+template <class E> struct Vec8;
+template <> struct Vec8<__bf16> { typedef bf16x8 t; };
+template <> struct Vec8<_Float16> { typedef f16x8 t; };
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ float trunc_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
 template <class T>
-__device__ __forceinline__ void pieces(T v, typename Mat<T>::e out[Mat<T>::P]) {
-    if constexpr (Mat<T>::P == 1) out[0] = v;
+__device__ __forceinline__ void pieces(float v, typename Mat<T>::e out[Mat<T>::P]) {
+    if constexpr (Mat<T>::P == 1) out[0] = (typename Mat<T>::e)v;
     else {
         const bool ok = __builtin_isfinite(v);              // an infinity or a NaN travels in the first piece alone
         const float a = ok ? trunc_bf16(v) : v, r = ok ? v - a : 0.0f, b = trunc_bf16(r);
@@ -54,128 +53,292 @@ __device__ __forceinline__ void pieces(T v, typename Mat<T>::e out[Mat<T>::P]) {
     }
 }
 
-// ------------------------------------------------------------------------------------------------ one product, any layout
-// C[m][n] = sum_k A(m, k) B(n, k):  A(m, k) = a[m lda + k] (AK 1) or a[k lda + m] (AK 0), B likewise.
-enum { EPI_OUT = 0, EPI_GATE = 1, EPI_DH = 2 };
-struct Prod {
-    const void* a; const void* b; int64_t lda, ldb;
-    int64_t M, N, K;
-    // EPI_OUT: out[m][n] = acc + bias[n] in T, or with `part` the fp32 share of a split over k: part[z][m][n]
-    void* out; const void* bias; float* part; int64_t k_per_split;
-    // EPI_GATE: N = H; B rows n (gate) and H + n (up); out = h [M][H], bias = b12, p / q fp32 or null.  EPI_DH: out = [dg | du] [M][2H]
-    float* p; float* q; int act;
-};
+// A row-major operand as the tile kernel reads it: planes of [rows][ld] elements, ld a multiple of 8, 16-byte aligned; the columns behind
+// its width (fewer than 8) are zero.  A 16-bit tensor of such a shape is its own operand; any other is packed into the workspace first.
+struct Operand { const void* p; int64_t ld, plane; };
 
-// 128 x 128 tiles, 32 deep, four waves of 64 x 64, tiles staged through registers element by element with bounds checks
-template <class T, int AK, int BK, int EPI>
-__global__ void __launch_bounds__(256) k_ffn_product(Prod g, int tiles_n) {
+// four consecutive values of a row as operand planes / as T
+template <class T>
+__device__ __forceinline__ void store_planes(typename Mat<T>::e* o, int64_t plane, const float v[4]) {
     typedef typename Mat<T>::e E;
-    typedef typename V8<E>::t E8;
-    constexpr int P = Mat<T>::P, LD = 40;
-    __shared__ __attribute__((aligned(16))) E sA[P][128][LD], sB[P][128][LD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
-    const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
-    const int64_t tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
-    constexpr int NT = EPI == EPI_GATE ? 64 : 128;             // columns of C a tile covers (a gate tile: 64 gate + 64 up)
-    const int64_t m0 = tm * 128, n0 = tn * NT;
-    const int64_t k_lo = blockIdx.y * g.k_per_split, k_hi = min(g.K, k_lo + g.k_per_split);
-    const T* const A = reinterpret_cast<const T*>(g.a);
-    const T* const B = reinterpret_cast<const T*>(g.b);
-    f32x16 acc[2][2];
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    constexpr int P = Mat<T>::P;
+    E4 t[P];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int i = 0; i < 4; ++i) {
+        E e[P];
+        pieces<T>(v[i], e);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
-    // column n of C that row r of the B tile holds, and whether it is an up row
-    auto b_row = [&](int r, int64_t& n) -> int64_t {
-        if (EPI != EPI_GATE) { n = n0 + r; return n; }
-        n = n0 + (r >> 6) * 32 + (r & 31);
-        return n + ((r >> 5) & 1) * g.N;
-    };
-    for (int64_t k0 = k_lo; k0 < k_hi; k0 += 32) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            E e[P];
-            {
-                const int r = AK ? (tid >> 5) + 8 * i : tid & 127, k = AK ? tid & 31 : (tid >> 7) + 2 * i;
-                const int64_t m = m0 + r, kk = k0 + k;
-                T v = (T)0.0f;
-                if (m < g.M && kk < k_hi) v = A[AK ? m * g.lda + kk : kk * g.lda + m];
-                pieces<T>(v, e);
-#pragma unroll
-                for (int p = 0; p < P; ++p) sA[p][r][k] = e[p];
-            }
-            {
-                const int r = BK ? (tid >> 5) + 8 * i : tid & 127, k = BK ? tid & 31 : (tid >> 7) + 2 * i;
-                int64_t n;
-                const int64_t row = b_row(r, n), kk = k0 + k;
-                T v = (T)0.0f;
-                if (n < g.N && kk < k_hi) v = B[BK ? row * g.ldb + kk : kk * g.ldb + row];
-                pieces<T>(v, e);
-#pragma unroll
-                for (int p = 0; p < P; ++p) sB[p][r][k] = e[p];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            E8 fa[P][2], fb[P][2];
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    fa[p][j] = *reinterpret_cast<const E8*>(&sA[p][wm + 32 * j + lr][16 * ks + 8 * lh]);
-                    fb[p][j] = *reinterpret_cast<const E8*>(&sB[p][wn + 32 * j + lr][16 * ks + 8 * lh]);
-                }
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    if constexpr (P == 3) {
-                        acc[a][b] = mfma(fb[2][a], fa[0][b], acc[a][b]);
-                        acc[a][b] = mfma(fb[0][a], fa[2][b], acc[a][b]);
-                        acc[a][b] = mfma(fb[1][a], fa[1][b], acc[a][b]);
-                        acc[a][b] = mfma(fb[1][a], fa[0][b], acc[a][b]);
-                        acc[a][b] = mfma(fb[0][a], fa[1][b], acc[a][b]);
-                    }
-                    acc[a][b] = mfma(fb[0][a], fa[0][b], acc[a][b]);
-                }
-        }
+        for (int p = 0; p < P; ++p) t[p][i] = e[p];
     }
-    // a lane holds row m = lr of C and columns (reg & 3) + 8 (reg >> 2) + 4 lh of each 32 x 32 block
-    const T* const bias = reinterpret_cast<const T*>(g.bias);
-    T* const out = reinterpret_cast<T*>(g.out);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int64_t m = m0 + wm + 32 * b + lr;
-        if (m >= g.M) continue;
-        if constexpr (EPI == EPI_GATE) {
+    for (int p = 0; p < P; ++p) *reinterpret_cast<E4*>(o + p * plane) = t[p];
+}
+template <class T>
+__device__ __forceinline__ void store4(T* o, const float v[4]) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<T4*>(o) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+}
+
+__host__ __device__ constexpr int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind column C and behind row R of a half; 8 columns per thread
+template <class T>
+__global__ void __launch_bounds__(256) k_ffn_pack(const T* __restrict__ src, int64_t R, int64_t RP, int64_t C, int64_t CP, int64_t rows_out, bool vec,
+                                                  typename Mat<T>::e* __restrict__ dst) {
+    typedef typename Mat<T>::e E;
+    typedef typename Vec8<E>::t E8;
+    constexpr int P = Mat<T>::P;
+    const int64_t cols8 = CP / 8, n = rows_out * cols8;
+    for (int64_t t = blockIdx.x * (int64_t)256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+        const int64_t row = t / cols8, c0 = (t - row * cols8) * 8;
+        const int64_t half = row / RP, r = row - half * RP;
+        float v[8];
+        const T* s = src + (half * R + r) * C + c0;
+        if (vec && r < R) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t n = n0 + (wn >> 6) * 32 + (r & 3) + 8 * (r >> 2) + 4 * lh;
-                if (n >= g.N) continue;
-                const float gv = acc[0][b][r] + (bias ? (float)bias[n] : 0.0f), uv = acc[1][b][r] + (bias ? (float)bias[g.N + n] : 0.0f);
-                float f, df;
-                activation<Mat<T>::P == 3>(g.act, gv, f, df);
-                out[m * g.N + n] = (T)(f * uv);
-                if (g.p) { g.p[m * g.N + n] = uv * df; g.q[m * g.N + n] = f; }
-            }
+            for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) Pack<T, 16 / sizeof(T)>::load(s + i, v + i);
         } else {
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int i = 0; i < 8; ++i) v[i] = r < R && c0 + i < C ? (float)s[i] : 0.0f;
+        }
+        E8 o[P];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int64_t n = n0 + wn + 32 * a + (r & 3) + 8 * (r >> 2) + 4 * lh;
-                    if (n >= g.N) continue;
-                    const float v = acc[a][b][r];
+        for (int i = 0; i < 8; ++i) {
+            E e[P];
+            pieces<T>(v[i], e);
+#pragma unroll
+            for (int p = 0; p < P; ++p) o[p][i] = e[p];
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) *reinterpret_cast<E8*>(dst + p * rows_out * CP + row * CP + c0) = o[p];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the tile kernel
+// C[m][n] = sum_k A(m, k) B(n, k).  KC: an operand's rows are m (or n) and its columns k; KS: its rows are k and its columns m (or n).
+enum { KC = 0, KS = 1 };
+enum { EPI_OUT = 0, EPI_GATE = 1, EPI_DH = 2 };
+struct Prod {
+    Operand a, b;
+    int64_t ra, rb;                       // rows of a KC operand (reads are clamped to them)
+    int64_t M, N, K, k_per_split;
+    // EPI_OUT: out[row(m)][n] = acc + bias[n], ld N; row(m) = m, or with two halves of `half_pad` padded rows each, of which `half` exist.
+    // With `part`: the fp32 share of a split over k instead, part[z][row][n] of rows_out rows
+    void* out; const void* bias; float* part; int64_t half_pad, half, rows_out; bool vec_out;
+    // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld HP = pad8(H); factors p, q [M][HP] or null; bias b12
+    // EPI_DH: out = [dg | du] planes of ld 2 HP
+    int64_t up_row, HP; float* p; float* q; int act;
+};
+
+__device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
+
+// Workgroups are dealt round-robin over the 8 XCDs, each with its own L2.  The ones that share an XCD (ids equal mod 8) take a contiguous
+// range of tiles, and that range runs down columns of 8 tiles of m before it moves on in n: what is in flight on an XCD shares operands.
+__device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, unsigned& tm, unsigned& tn) {
+    const unsigned total = gm * gn, xcd = id & 7, q = total >> 3, r = total & 7;
+    unsigned t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
+    const unsigned group = t / (8 * gn), first = group * 8, rows = min(gm - first, 8u);
+    t -= group * 8 * gn;
+    tm = first + t % rows;
+    tn = t / rows;
+}
+
+// Tiles of 32 MR WM x 32 NR WN, 64 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
+// 1 KB per instruction, lane-linear in LDS) into two buffers: step t + 1 travels while step t is multiplied.  A KC tile is rows of 64 k
+// (128 B), its 16-byte chunk c in slot c ^ (row / 2 & 7); a KS tile is rows of one k (64 or 128 chunks of m), chunk c in slot
+// c ^ 4 (k & 3), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
+// keep every LDS read free of bank conflicts.
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR>
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
+    typedef typename Mat<T>::e E;
+    typedef typename Vec8<E>::t E8;
+    constexpr int P = Mat<T>::P, NW = WM * WN, BM = 32 * MR * WM, BN = 32 * NR * WN;
+    constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;                 // 1-KB pieces per wave and step
+    constexpr int TILE = (BM + BN) * 128;
+    __shared__ __attribute__((aligned(1024))) char s_all[2 * TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, lh = lane >> 5;
+    const int wm = (wave / WN) * 32 * MR, wn = (wave % WN) * 32 * NR;
+    unsigned tm, tn;
+    tile_of(blockIdx.x, gm, gn, tm, tn);
+    constexpr int NT = EPI == EPI_GATE ? BN / 2 : BN;                 // columns of C per tile (a gate tile: as many gate as up columns)
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * NT;
+    const int64_t k_lo = blockIdx.y * g.k_per_split, k_hi = min(g.K, k_lo + g.k_per_split);
+    const E* const A = reinterpret_cast<const E*>(g.a.p);
+    const E* const B = reinterpret_cast<const E*>(g.b.p);
+
+    // the lane's source of each piece, in bytes from the tile's corner at the step's k (ld < 2^22: 256 rows stay below 2^31), and its first k
+    uint32_t oa[PA], ob[PB];
+    int ka[PA], kb[PB];
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+        const int at = (wave + NW * i) * 1024 + lane * 16;
+        const int r = at / (AK == KC ? 128 : BM * 2), c = ((at % (AK == KC ? 128 : BM * 2)) >> 4) ^ (AK == KC ? (r >> 1) & 7 : (r & 3) << 2);
+        if (AK == KC) { oa[i] = (uint32_t)((min(m0 + r, g.ra - 1) - m0) * g.a.ld + c * 8) * 2; ka[i] = c * 8; }
+        else { oa[i] = (uint32_t)(r * g.a.ld + min(m0 + c * 8, g.a.ld - 8) - m0) * 2; ka[i] = r; }
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+        const int at = (wave + NW * i) * 1024 + lane * 16;
+        const int r = at / (BK == KC ? 128 : BN * 2), c = ((at % (BK == KC ? 128 : BN * 2)) >> 4) ^ (BK == KC ? (r >> 1) & 7 : (r & 3) << 2);
+        if (BK == KC) {
+            // a gate tile's rows: 32 gate rows, the 32 up rows of the same hidden units, the next 32 gate rows ...
+            const int64_t row = EPI == EPI_GATE ? min(n0 + (r >> 6) * 32 + (r & 31), g.N - 1) : min(n0 + r, g.rb - 1);
+            ob[i] = (uint32_t)((row - n0) * g.b.ld + c * 8) * 2;
+            kb[i] = c * 8;
+        } else { ob[i] = (uint32_t)(r * g.b.ld + min(n0 + c * 8, g.b.ld - 8) - n0) * 2; kb[i] = r; }
+    }
+    const int64_t sa = AK == KC ? 64 : 64 * g.a.ld, sb = BK == KC ? 64 : 64 * g.b.ld;            // elements per step
+    const E* const a0 = A + (AK == KC ? m0 * g.a.ld + k_lo : k_lo * g.a.ld + m0);
+    const E* const b0 = B + (BK == KC ? n0 * g.b.ld + k_lo : k_lo * g.b.ld + n0);
+    const int steps_k = (int)((k_hi - k_lo + 63) / 64), steps = k_hi > k_lo ? steps_k * (P == 3 ? 6 : 1) : 0;
+
+    auto issue = [&](int pair, int kt, int buf) {
+        // planes of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+        const int pa = P == 1 ? 0 : pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = P == 1 ? 0 : pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
+        const char* as = reinterpret_cast<const char*>(a0 + pa * g.a.plane + kt * sa);
+        const char* bs = reinterpret_cast<const char*>(b0 + pb * g.b.plane + kt * sb);
+        char* dst = s_all + buf * TILE + wave * 1024;
+        const int64_t left = k_hi - k_lo - (int64_t)kt * 64;          // k values from this step on
+        const auto load = [&](const char* src, char* to) {
+            __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+        };
+        const auto b_base = [&](int i) { return EPI == EPI_GATE && (((wave + NW * i) >> 2) & 1) ? bs + g.up_row * g.b.ld * 2 : bs; };
+        if (left >= 64) {
+#pragma unroll
+            for (int i = 0; i < PA; ++i) load(as + oa[i], dst + i * NW * 1024);
+#pragma unroll
+            for (int i = 0; i < PB; ++i) load(b_base(i) + ob[i], dst + BM * 128 + i * NW * 1024);
+        } else {                                                      // the last, partly filled step: zeros behind k_hi
+            const char* const zero = reinterpret_cast<const char*>(g_zeros);
+#pragma unroll
+            for (int i = 0; i < PA; ++i) load(ka[i] < left ? as + oa[i] : zero, dst + i * NW * 1024);
+#pragma unroll
+            for (int i = 0; i < PB; ++i) load(kb[i] < left ? b_base(i) + ob[i] : zero, dst + BM * 128 + i * NW * 1024);
+        }
+    };
+
+    // where this lane's fragments are in a tile: KC one 16-byte read per 16 k, KS two transposed 8-byte reads
+    constexpr int ROWA = AK == KC ? 128 : BM * 2, ROWB = BK == KC ? 128 : BN * 2;
+    const int sw = (lr >> 1) & 7, trow = 8 * lh + ((lane & 15) >> 2), tx = ((lane >> 2) & 3) << 2;
+    const int tcol = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+    auto frag = [&](const char* tile, int kind, int rowbytes, int base, int j, int ks) -> E8 {
+        if (kind == KC) return *reinterpret_cast<const E8*>(tile + (base + 32 * j + lr) * 128 + (((2 * ks + lh) ^ sw) << 4));
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const char* at = tile + (16 * ks + trow) * rowbytes + (((base / 8 + 4 * j) ^ tx) << 4) + tcol;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 4 * rowbytes));
+        const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return __builtin_bit_cast(E8, v);
+    };
+
+    f32x16 acc[NR][MR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[n][m][r] = 0.0f;
+    int pair = 0, kt = 0;
+    if (steps) issue(0, 0, 0);
+    for (int t = 0; t < steps; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // this wave's pieces of step t have landed ...
+        __builtin_amdgcn_s_barrier();                                 // ... everybody's have, and everybody has read step t - 1
+        asm volatile("" ::: "memory");
+        if (++kt == steps_k) { kt = 0; ++pair; }
+        if (t + 1 < steps) issue(pair, kt, (t + 1) & 1);
+        const char* const ta = s_all + (t & 1) * TILE;
+        const char* const tb = ta + BM * 128;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            E8 fa[MR], fb[NR];
+#pragma unroll
+            for (int j = 0; j < NR; ++j) fb[j] = frag(tb, BK, ROWB, wn, j, ks);
+#pragma unroll
+            for (int j = 0; j < MR; ++j) fa[j] = frag(ta, AK, ROWA, wm, j, ks);
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+#pragma unroll
+                for (int n = 0; n < NR; ++n) acc[n][m] = mfma(fb[n], fa[m], acc[n][m]);
+        }
+    }
+
+    // a lane holds row m = lr of C and columns (reg & 3) + 8 (reg >> 2) + 4 lh of each 32 x 32 block
+    const T* const bias = reinterpret_cast<const T*>(g.bias);
+#pragma unroll
+    for (int mb = 0; mb < MR; ++mb) {
+        const int64_t m = m0 + wm + 32 * mb + lr;
+        if (m >= g.M) continue;
+        if constexpr (EPI == EPI_GATE) {
+            static_assert(NR == 2, "a wave's columns are 32 gate and 32 up columns");
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const int64_t n = n0 + (wn >> 1) + 8 * q4 + 4 * lh;
+                if (n >= g.HP) continue;
+                float hv[4], pv[4], qv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = n + i < g.N;
+                    const float gv = acc[0][mb][4 * q4 + i] + (in && bias ? (float)bias[n + i] : 0.0f);
+                    const float uv = acc[1][mb][4 * q4 + i] + (in && bias ? (float)bias[g.N + n + i] : 0.0f);
+                    float f, df;
+                    activation<P == 3>(g.act, gv, f, df);
+                    hv[i] = in ? f * uv : 0.0f;
+                    pv[i] = in ? uv * df : 0.0f;
+                    qv[i] = in ? f : 0.0f;
+                }
+                store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.HP + n, g.M * g.HP, hv);
+                if (g.p) {
+                    Pack<float, 4>::store(g.p + m * g.HP + n, pv);
+                    Pack<float, 4>::store(g.q + m * g.HP + n, qv);
+                }
+            }
+        } else {
+            int64_t row = m;
+            if (EPI == EPI_OUT && g.half_pad) {
+                const int64_t hf = m >= g.half_pad;
+                if (m - hf * g.half_pad >= g.half) continue;
+                row = hf * g.half + m - hf * g.half_pad;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NR; ++nb)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const int64_t n = n0 + wn + 32 * nb + 8 * q4 + 4 * lh;
+                    float v[4] = {acc[nb][mb][4 * q4], acc[nb][mb][4 * q4 + 1], acc[nb][mb][4 * q4 + 2], acc[nb][mb][4 * q4 + 3]};
                     if constexpr (EPI == EPI_DH) {
-                        out[m * 2 * g.N + n] = (T)(v * g.p[m * g.N + n]);
-                        out[m * 2 * g.N + g.N + n] = (T)(v * g.q[m * g.N + n]);
-                    } else if (g.part) g.part[(blockIdx.y * g.M + m) * g.N + n] = v;
-                    else out[m * g.N + n] = (T)(v + (bias ? (float)bias[n] : 0.0f));
+                        if (n >= g.HP) continue;
+                        float p[4], q[4];
+                        Pack<float, 4>::load(g.p + m * g.HP + n, p);
+                        Pack<float, 4>::load(g.q + m * g.HP + n, q);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool in = n + i < g.N;
+                            p[i] = in ? v[i] * p[i] : 0.0f;
+                            q[i] = in ? v[i] * q[i] : 0.0f;
+                        }
+                        E* o = reinterpret_cast<E*>(g.out) + m * 2 * g.HP + n;
+                        store_planes<T>(o, g.M * 2 * g.HP, p);
+                        store_planes<T>(o + g.HP, g.M * 2 * g.HP, q);
+                    } else if (g.part) {
+                        float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
+                        if (g.vec_out && n < g.N) Pack<float, 4>::store(o, v);
+                        else
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (n + i < g.N) o[i] = v[i];
+                    } else {
+                        T* o = reinterpret_cast<T*>(g.out) + row * g.N + n;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (bias && n + i < g.N) v[i] += (float)bias[n + i];
+                        if (g.vec_out && n < g.N) store4<T>(o, v);
+                        else
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (n + i < g.N) o[i] = (T)v[i];
+                    }
                 }
         }
     }
@@ -191,115 +354,195 @@ __global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part
     }
 }
 
-// column sums of a [M][N] matrix: part[y][n] over the rows y, y + gridDim.y, ...; k_ffn_join adds the shares
-template <class T>
-__global__ void __launch_bounds__(256) k_ffn_colsum(const T* __restrict__ a, int64_t M, int64_t N, float* __restrict__ part) {
+// column sums of [M][ld] planes over the rows y, y + gridDim.y, ...: part[y][column]; with halves of half_pad padded columns the pads are
+// left out.  k_ffn_join adds the shares
+template <class S, int P>
+__global__ void __launch_bounds__(256) k_ffn_colsum(const S* __restrict__ a, int64_t ld, int64_t plane, int64_t M, int64_t N, int64_t half_pad,
+                                                    int64_t half, float* __restrict__ part) {
     const int64_t n = blockIdx.x * (int64_t)256 + threadIdx.x;
     if (n >= N) return;
+    const int64_t c = half_pad && n >= half ? n - half + half_pad : n;
     float v = 0.0f;
-    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) v += (float)a[m * N + n];
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y)
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) v += (float)a[p * plane + m * ld + c];
     part[blockIdx.y * N + n] = v;
 }
 
 // ------------------------------------------------------------------------------------------------ launches
 constexpr int CSUM = 64;                                         // shares of a column sum
 
-// shares of a product's k loop when its tiles alone do not fill the chip; each at least 256 deep
-inline int k_splits(int64_t M, int64_t N, int64_t K) {
-    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), (K + 255) / 256, 64}));
+inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// the workspace, handed out front to back; with base null only its size is counted and nothing is launched
+struct Work {
+    char* base; size_t used; hipStream_t s;
+    void* take(size_t bytes) { void* p = base ? base + used : nullptr; used += up256(bytes); return p; }
+    bool counting() const { return !base; }
+};
+#define FFN_TRY(call) do { const hipError_t e__ = (call); if (e__ != hipSuccess) return e__; } while (0)
+
+template <class T> inline size_t planes_bytes(int64_t rows, int64_t ld) { return (size_t)rows * ld * Mat<T>::P * 2; }
+
+// src [halves x R][C] as an operand: itself, or packed
+template <class T>
+hipError_t operand(Work& w, const void* src, int64_t halves, int64_t R, int64_t C, Operand& o) {
+    const int64_t RP = halves > 1 ? pad8(R) : R, CP = pad8(C), rows = halves * RP;
+    o.ld = CP; o.plane = rows * CP; o.p = src;
+    if (Mat<T>::P == 1 && CP == C && RP == R && (w.counting() || aligned16(src))) {
+        // (counting: a start that is not 16-byte aligned is copied too, and the size must not depend on it)
+        if (w.counting()) w.take(planes_bytes<T>(rows, CP));
+        return hipSuccess;
+    }
+    void* dst = w.take(planes_bytes<T>(rows, CP));
+    o.p = dst;
+    if (w.counting() || rows == 0) return hipSuccess;
+    const int64_t n = rows * CP / 8;
+    k_ffn_pack<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192), 256, 0, w.s>>>((const T*)src, R, RP, C, CP, rows, aligned16(src) && CP == C,
+                                                                                       (typename Mat<T>::e*)dst);
+    return hipGetLastError();
 }
 
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR>
+hipError_t tiles(Prod g, int splits, hipStream_t s) {
+    constexpr int BM = 32 * MR * WM, NT = EPI == EPI_GATE ? 16 * NR * WN : 32 * NR * WN;
+    const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M + BM - 1) / BM, gn = (N + NT - 1) / NT;
+    if (!gm || !gn) return hipSuccess;
+    if (gm * gn > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 63) / 64 * 64 : std::max<int64_t>(g.K, 64);
+    k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
+    return hipGetLastError();
+}
+inline int64_t tile_count(int64_t M, int64_t N, int side) { return ((M + side - 1) / side) * ((N + side - 1) / side); }
+
+// 256 x 256 tiles (8 waves) where they fill the chip, else 128 x 128 (4 waves)
 template <class T, int AK, int BK, int EPI>
-hipError_t product(Prod g, int splits, hipStream_t s) {
-    const int nt = EPI == EPI_GATE ? 64 : 128;
-    const int64_t tn = (g.N + nt - 1) / nt, tm = (g.M + 127) / 128;
-    if (!tm || !tn) return hipSuccess;
-    g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 31) / 32 * 32 : std::max<int64_t>(g.K, 1);
-    k_ffn_product<T, AK, BK, EPI><<<dim3((unsigned)(tm * tn), splits), 256, 0, s>>>(g, (int)tn);
-    return hipGetLastError();
+hipError_t product(const Prod& g, int splits, hipStream_t s) {
+    const int64_t N = EPI == EPI_GATE ? 2 * g.HP : EPI == EPI_DH ? g.HP : g.N;
+    if (tile_count(g.M, N, 256) * splits >= 192) return tiles<T, AK, BK, EPI, 2, 4, 4, 2>(g, splits, s);
+    return tiles<T, AK, BK, EPI, 2, 2, 2, 2>(g, splits, s);
 }
-template <class T, int AK, int BK>
-hipError_t product_split(Prod g, float* part, hipStream_t s) {
+
+// shares of a weight gradient's sum over the rows, when its tiles alone do not fill the chip: each at least 512 deep
+inline int k_splits(int64_t M, int64_t N, int64_t K) {
+    const int64_t t = tile_count(M, N, 128);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(t, 1), K / 512, 64}));
+}
+template <class T>
+hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
     const int z = k_splits(g.M, g.N, g.K);
-    if (z == 1) return product<T, AK, BK, EPI_OUT>(g, 1, s);
-    g.part = part;
-    hipError_t e = product<T, AK, BK, EPI_OUT>(g, z, s);
-    if (e != hipSuccess) return e;
-    const int64_t n = g.M * g.N;
-    k_ffn_join<T><<<(int)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, s>>>(part, z, n, (T*)g.out);
+    g.rows_out = rows_out;
+    if (z > 1) g.part = (float*)w.take((size_t)z * rows_out * g.N * 4);
+    if (w.counting()) return hipSuccess;
+    g.vec_out = g.N % 4 == 0 && (z > 1 || aligned16(g.out));
+    FFN_TRY((product<T, KS, KS, EPI_OUT>(g, z, w.s)));
+    if (z == 1) return hipSuccess;
+    const int64_t n = rows_out * g.N;
+    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, w.s>>>(g.part, z, n, (T*)g.out);
     return hipGetLastError();
 }
-template <class T>
-hipError_t colsum(const void* a, int64_t M, int64_t N, float* part, void* out, hipStream_t s) {
-    k_ffn_colsum<T><<<dim3((unsigned)((N + 255) / 256), CSUM), 256, 0, s>>>((const T*)a, M, N, part);
-    k_ffn_join<T><<<(int)((N + 255) / 256), 256, 0, s>>>(part, CSUM, N, (T*)out);
+template <class T, class S, int P>
+hipError_t colsum(Work& w, const void* a, int64_t ld, int64_t plane, int64_t M, int64_t N, int64_t half_pad, int64_t half, void* out) {
+    float* part = (float*)w.take((size_t)CSUM * N * 4);
+    if (w.counting()) return hipSuccess;
+    k_ffn_colsum<S, P><<<dim3((unsigned)((N + 255) / 256), CSUM), 256, 0, w.s>>>((const S*)a, ld, plane, M, N, half_pad, half, part);
+    k_ffn_join<T><<<(unsigned)((N + 255) / 256), 256, 0, w.s>>>(part, CSUM, N, (T*)out);
     return hipGetLastError();
 }
 
+// what the forward pass keeps: h planes, then p and q
+template <class T> inline size_t kept_h(int64_t M, int64_t H) { return up256(planes_bytes<T>(M, pad8(H))); }
+
 template <class T>
-hipError_t forward(const FfnArgs& f, void* ws, hipStream_t s) {
+hipError_t forward(const FfnArgs& f, Work& w) {
+    const int64_t HP = pad8(f.H);
+    Operand x, w12, w3;
+    FFN_TRY(operand<T>(w, f.x, 1, f.M, f.D, x));
+    FFN_TRY(operand<T>(w, f.w12, 2, f.H, f.D, w12));
+    FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
+    char* h = (char*)f.kept;
+    if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
+    if (w.counting()) return hipSuccess;
     Prod g{};
-    g.a = f.x; g.lda = f.D; g.b = f.w12; g.ldb = f.D; g.M = f.M; g.N = f.H; g.K = f.D;
-    g.out = f.h ? f.h : ws; g.bias = f.b12; g.act = f.act;
-    if (f.pq) { g.p = f.pq; g.q = f.pq + f.M * f.H; }
-    hipError_t e = product<T, 1, 1, EPI_GATE>(g, 1, s);
-    if (e != hipSuccess) return e;
+    g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.up_row = HP;
+    if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
+    FFN_TRY((product<T, KC, KC, EPI_GATE>(g, 1, w.s)));
     Prod d{};
-    d.a = g.out; d.lda = f.H; d.b = f.w3; d.ldb = f.H; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
-    return product<T, 1, 1, EPI_OUT>(d, 1, s);
+    d.a = {h, HP, f.M * HP}; d.b = w3; d.ra = f.M; d.rb = f.O; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
+    d.vec_out = f.O % 4 == 0 && aligned16(f.y);
+    return product<T, KC, KC, EPI_OUT>(d, 1, w.s);
 }
 
 template <class T>
-hipError_t backward(const FfnArgs& f, void* ws, hipStream_t s) {
-    T* const dgu = reinterpret_cast<T*>(ws);
-    float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + ((size_t)f.M * 2 * f.H * sizeof(T) + 255) / 256 * 256);
-    hipError_t e = hipSuccess;
-    if (f.dx || f.dw12 || f.db12) {
-        Prod g{};
-        g.a = f.dy; g.lda = f.O; g.b = f.w3; g.ldb = f.H; g.M = f.M; g.N = f.H; g.K = f.O; g.out = dgu; g.p = f.pq; g.q = f.pq + f.M * f.H;
-        if ((e = product<T, 1, 0, EPI_DH>(g, 1, s)) != hipSuccess) return e;
+hipError_t backward(const FfnArgs& f, Work& w) {
+    typedef typename Mat<T>::e E;
+    constexpr int P = Mat<T>::P;
+    const int64_t HP = pad8(f.H);
+    const bool all = w.counting(), hidden = all || f.dx || f.dw12 || f.db12;
+    char* h = (char*)f.kept;
+    const float* p = (const float*)(h + (all ? 0 : kept_h<T>(f.M, f.H)));
+    Operand dy{};
+    if (hidden || f.dw3) FFN_TRY(operand<T>(w, f.dy, 1, f.M, f.O, dy));
+    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
+    if (hidden) {
+        Operand w3;
+        FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
+        if (!all) {
+            Prod g{};
+            g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP;
+            g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
+            FFN_TRY((product<T, KC, KS, EPI_DH>(g, 1, w.s)));
+        }
     }
-    if (f.dx) {
-        Prod g{};
-        g.a = dgu; g.lda = 2 * (int64_t)f.H; g.b = f.w12; g.ldb = f.D; g.M = f.M; g.N = f.D; g.K = 2 * (int64_t)f.H; g.out = f.dx;
-        if ((e = product<T, 1, 0, EPI_OUT>(g, 1, s)) != hipSuccess) return e;
+    if (all || f.dx) {
+        Operand w12;
+        FFN_TRY(operand<T>(w, f.w12, 2, f.H, f.D, w12));
+        if (!all) {
+            Prod g{};
+            g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
+            FFN_TRY((product<T, KC, KS, EPI_OUT>(g, 1, w.s)));
+        }
     }
-    if (f.dw12) {
+    if (all || f.dw12) {
+        Operand x;
+        FFN_TRY(operand<T>(w, f.x, 1, f.M, f.D, x));
         Prod g{};
-        g.a = dgu; g.lda = 2 * (int64_t)f.H; g.b = f.x; g.ldb = f.D; g.M = 2 * (int64_t)f.H; g.N = f.D; g.K = f.M; g.out = f.dw12;
-        if ((e = product_split<T, 0, 0>(g, part, s)) != hipSuccess) return e;
+        g.a = dgu; g.b = x; g.M = 2 * HP; g.N = f.D; g.K = f.M; g.out = f.dw12; g.half_pad = HP; g.half = f.H;
+        FFN_TRY(weight_gradient<T>(w, g, 2 * (int64_t)f.H));
     }
-    if (f.dw3) {
+    if (all || f.dw3) {
         Prod g{};
-        g.a = f.dy; g.lda = f.O; g.b = f.h; g.ldb = f.H; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
-        if ((e = product_split<T, 0, 0>(g, part, s)) != hipSuccess) return e;
+        g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
+        FFN_TRY(weight_gradient<T>(w, g, f.O));
     }
-    if (f.db12 && (e = colsum<T>(dgu, f.M, 2 * (int64_t)f.H, part, f.db12, s)) != hipSuccess) return e;
-    if (f.db3 && (e = colsum<T>(f.dy, f.M, f.O, part, f.db3, s)) != hipSuccess) return e;
+    if (all || f.db12) FFN_TRY((colsum<T, E, P>(w, dgu.p, 2 * HP, dgu.plane, f.M, 2 * (int64_t)f.H, HP, f.H, f.db12)));
+    if (all || f.db3) FFN_TRY((colsum<T, T, 1>(w, f.dy, f.O, 0, f.M, f.O, 0, 0, f.db3)));
     return hipSuccess;
 }
 
-inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+template <class F>
+auto by_type(int dt, F f) { return dt == IFF_DT_F32 ? f(float{}) : dt == IFF_DT_BF16 ? f(__bf16{}) : f(_Float16{}); }
 
 }  // namespace
 
-size_t ffn_forward_workspace(const FfnArgs& a, bool keeps_h) { return keeps_h ? 0 : up256((size_t)a.M * a.H * dt_size(a.dt)); }
-
-size_t ffn_backward_workspace(const FfnArgs& a) {
-    size_t part = std::max((size_t)CSUM * 2 * a.H * 4, (size_t)CSUM * a.O * 4);
-    const auto split = [&](int64_t M, int64_t N) {
-        const int z = k_splits(M, N, a.M);
-        if (z > 1) part = std::max(part, (size_t)z * M * N * 4);
-    };
-    split(2 * (int64_t)a.H, a.D);
-    split(a.O, a.H);
-    return up256((size_t)a.M * 2 * a.H * dt_size(a.dt)) + up256(part);
+size_t ffn_kept_bytes(const FfnArgs& a) {
+    return by_type(a.dt, [&](auto t) { return kept_h<decltype(t)>(a.M, a.H) + (size_t)2 * a.M * pad8(a.H) * 4; });
 }
-
+size_t ffn_forward_workspace(const FfnArgs& a) {
+    Work w{nullptr, 0, nullptr};
+    (void)by_type(a.dt, [&](auto t) { return forward<decltype(t)>(a, w); });
+    return w.used;
+}
+size_t ffn_backward_workspace(const FfnArgs& a) {
+    Work w{nullptr, 0, nullptr};
+    (void)by_type(a.dt, [&](auto t) { return backward<decltype(t)>(a, w); });
+    return w.used;
+}
 hipError_t launch_ffn_forward(const FfnArgs& a, void* ws, hipStream_t s) {
-    return a.dt == IFF_DT_F32 ? forward<float>(a, ws, s) : a.dt == IFF_DT_BF16 ? forward<__bf16>(a, ws, s) : forward<_Float16>(a, ws, s);
+    Work w{(char*)ws, 0, s};
+    return by_type(a.dt, [&](auto t) { return forward<decltype(t)>(a, w); });
 }
 hipError_t launch_ffn_backward(const FfnArgs& a, void* ws, hipStream_t s) {
-    return a.dt == IFF_DT_F32 ? backward<float>(a, ws, s) : a.dt == IFF_DT_BF16 ? backward<__bf16>(a, ws, s) : backward<_Float16>(a, ws, s);
+    Work w{(char*)ws, 0, s};
+    return by_type(a.dt, [&](auto t) { return backward<decltype(t)>(a, w); });
 }

@@ -159,27 +159,26 @@ def _mlp_forward(x, w12, b12, w3, b3, act, keep):
     M, D = x.shape
     O, H = w3.shape
     ty = _TYPES[x.dtype]
+    L = _lib._lib or _lib.lib()
     y = x.new_empty((M, O))
-    h = x.new_empty((M, H)) if keep else None
-    pq = x.new_empty((2, M, H), dtype=torch.float32) if keep else None
-    nbytes = (_lib._lib or _lib.lib()).iff_gated_mlp_forward_workspace(ty, M, D, H, O, keep)
-    ws = _workspace(nbytes, x) if nbytes else None
+    kept = x.new_empty((L.iff_gated_mlp_kept_bytes(ty, M, D, H, O),), dtype=torch.uint8) if keep else None
+    ws = _workspace(L.iff_gated_mlp_forward_workspace(ty, M, D, H, O), x)
     _run("iff_gated_mlp_forward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), _ptr(b12), w3.data_ptr(), _ptr(b3), act, y.data_ptr(),
-         _ptr(h), _ptr(pq), _ptr(ws), nbytes)
-    return y, h, pq
+         _ptr(kept), kept.numel() if keep else 0, ws.data_ptr(), ws.numel())
+    return y, kept
 
 
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w12, b12, w3, b3, act):
-        y, h, pq = _mlp_forward(x, w12, b12, w3, b3, act, True)
-        ctx.save_for_backward(x, w12, w3, h, pq)
+        y, kept = _mlp_forward(x, w12, b12, w3, b3, act, True)
+        ctx.save_for_backward(x, w12, w3, kept)
         return y
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
-        x, w12, w3, h, pq = ctx.saved_tensors
+        x, w12, w3, kept = ctx.saved_tensors
         M, D = x.shape
         O, H = w3.shape
         ty, dy = _TYPES[x.dtype], dy.contiguous()
@@ -189,9 +188,8 @@ class _GatedMlp(torch.autograd.Function):
         db12 = x.new_empty((2 * H,)) if need[2] else None
         dw3 = x.new_empty((O, H)) if need[3] else None
         db3 = x.new_empty((O,)) if need[4] else None
-        nbytes = _lib._lib.iff_gated_mlp_backward_workspace(ty, M, D, H, O)
-        ws = _workspace(nbytes, x)
-        _run("iff_gated_mlp_backward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), h.data_ptr(), pq.data_ptr(),
+        ws = _workspace(_lib._lib.iff_gated_mlp_backward_workspace(ty, M, D, H, O), x)
+        _run("iff_gated_mlp_backward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), kept.data_ptr(),
              dy.data_ptr(), _ptr(dx), _ptr(dw12), _ptr(db12), _ptr(dw3), _ptr(db3), ws.data_ptr(), ws.numel())
         return dx, dw12, db12, dw3, db3, None
 

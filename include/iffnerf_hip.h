@@ -567,18 +567,19 @@ int iff_layer_norm_backward(const void* x, int32_t x_type, int64_t n0, int64_t n
 
 /* Gated feed-forward block (the MLP half of a backbone block, pose_estimation/backbone.py:12-14, in its gated form):
  *   [g | u] = x w12^T + b12,  h = act(g) u,  y = h w3^T + b3
- * x [M, D], w12 [2H, D] (gate rows first), w3 [O, H], b12_opt [2H], b3_opt [O], y [M, O]: one type, contiguous.  For the backward pass
- * h_opt [M, H] (same type) and factors_opt [2, M, H] fp32 = (u act'(g), act(g)) are kept -- both or neither.  Workspace:
- * iff_gated_mlp_forward_workspace (0 where h_opt is given may still be passed). */
-size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, int32_t keeps_h);
+ * x [M, D], w12 [2H, D] (gate rows first), w3 [O, H], b12_opt [2H], b3_opt [O], y [M, O]: one type, contiguous; D, 2H, O <= 2^21.
+ * kept_opt (iff_gated_mlp_kept_bytes, opaque) is what the backward pass reads of the hidden activation: h rounded to the type, and
+ * u act'(g) and act(g) in fp32.  Workspaces and kept are 16-byte aligned; a workspace is free again when the call's kernels have run. */
+size_t iff_gated_mlp_kept_bytes(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
+size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
 int iff_gated_mlp_forward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12, const void* b12_opt,
-                          const void* w3, const void* b3_opt, int32_t activation, void* y, void* h_opt, float* factors_opt, void* workspace,
+                          const void* w3, const void* b3_opt, int32_t activation, void* y, void* kept_opt, size_t kept_bytes, void* workspace,
                           size_t workspace_bytes, void* stream);
 /* Its gradients (autograd's backward in pose_estimation/train.py:119): dy [M, O] -> the outputs that are not NULL, in the operands' type. */
 size_t iff_gated_mlp_backward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
 int iff_gated_mlp_backward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12, const void* w3,
-                           const void* h, const float* factors, const void* dy, void* dx_opt, void* dw12_opt, void* db12_opt, void* dw3_opt,
-                           void* db3_opt, void* workspace, size_t workspace_bytes, void* stream);
+                           const void* kept, const void* dy, void* dx_opt, void* dw12_opt, void* db12_opt, void* dw3_opt, void* db3_opt,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* Dropout without a stored mask (the dropout of a backbone block under pose_estimation/train.py:97-119):
  *   y[i] = residual_opt[i] + (keep_i ? x[i] / (1 - p) : 0),  p = threshold / 65536

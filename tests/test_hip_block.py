@@ -606,16 +606,21 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
     refused(L.iff_layer_norm_backward(one, 0, 1, 4, 0, 4, 4, None, 0, one, one, one, one, None, None, 0, None), b"workspace")
     refused(L.iff_layer_norm_backward(None, 0, 1, 4, 0, 4, 4, None, 0, None, None, one, None, None, None, 0, None), b"null")
     assert L.iff_layer_norm_backward(None, 0, 1, 4, 0, 4, 4, None, 0, None, None, None, None, None, None, 0, None) == 0
-    refused(L.iff_gated_mlp_forward(None, 5, 1, 4, 4, 4, None, None, None, None, 0, None, None, None, None, 0, None), b"type 5")
-    refused(L.iff_gated_mlp_forward(None, 0, -1, 4, 4, 4, None, None, None, None, 0, None, None, None, None, 0, None), b"bad row count")
-    refused(L.iff_gated_mlp_forward(None, 0, 1, 4, 0, 4, None, None, None, None, 0, None, None, None, None, 0, None), b"bad widths")
-    refused(L.iff_gated_mlp_forward(None, 0, 1, 4, 4, 4, None, None, None, None, 7, None, None, None, None, 0, None), b"activation 7")
-    refused(L.iff_gated_mlp_forward(None, 0, 1, 4, 4, 4, None, None, None, None, 0, None, None, None, None, 0, None), b"null")
-    refused(L.iff_gated_mlp_forward(one, 0, 1, 4, 4, 4, one, None, one, None, 0, one, one, None, one, 1 << 20, None), b"together")
-    refused(L.iff_gated_mlp_forward(one, 0, 1, 4, 4, 4, one, None, one, None, 0, one, None, None, None, 0, None), b"workspace")
-    assert L.iff_gated_mlp_forward(None, 0, 0, 4, 4, 4, None, None, None, None, 0, None, None, None, None, 0, None) == 0
-    refused(L.iff_gated_mlp_backward(one, 0, 8, 4, 4, 4, one, one, one, one, one, one, None, None, None, None, None, 0, None), b"workspace")
-    refused(L.iff_gated_mlp_backward(None, 0, 8, 4, 4, 4, None, None, None, None, None, one, None, None, None, None, None, 0, None), b"null")
+    G, B = L.iff_gated_mlp_forward, L.iff_gated_mlp_backward
+    refused(G(None, 5, 1, 4, 4, 4, None, None, None, None, 0, None, None, 0, None, 0, None), b"type 5")
+    refused(G(None, 0, -1, 4, 4, 4, None, None, None, None, 0, None, None, 0, None, 0, None), b"bad row count")
+    refused(G(None, 0, 1, 4, 0, 4, None, None, None, None, 0, None, None, 0, None, 0, None), b"bad widths")
+    refused(G(None, 0, 1, 4, (1 << 20) + 1, 4, None, None, None, None, 0, None, None, 0, None, 0, None), b"bad widths")
+    refused(G(None, 0, 1, 4, 4, 4, None, None, None, None, 7, None, None, 0, None, 0, None), b"activation 7")
+    refused(G(None, 0, 1, 4, 4, 4, None, None, None, None, 0, None, None, 0, None, 0, None), b"null")
+    refused(G(one, 0, 1, 4, 4, 4, one, None, one, None, 0, one, one, 8, one, 1 << 20, None), b"kept 8")
+    refused(G(one, 0, 1, 4, 4, 4, one, None, one, None, 0, one, None, 0, None, 0, None), b"workspace 0")
+    refused(G(one, 0, 1, 4, 4, 4, one, None, one, None, 0, one, None, 0, 24, 1 << 20, None), b"aligned")
+    assert G(None, 0, 0, 4, 4, 4, None, None, None, None, 0, None, None, 0, None, 0, None) == 0
+    refused(B(one, 0, 8, 4, 4, 4, one, one, one, one, one, None, None, None, None, None, 0, None), b"workspace 0")
+    refused(B(None, 0, 8, 4, 4, 4, None, None, None, None, one, None, None, None, None, None, 0, None), b"null")
+    refused(B(one, 0, 8, 4, 4, 4, one, one, 24, one, one, None, None, None, None, one, 1 << 30, None), b"aligned")
+    assert L.iff_gated_mlp_kept_bytes(1, 8, 4, 4, 4) > 0 and L.iff_gated_mlp_kept_bytes(9, 8, 4, 4, 4) == 0
     refused(L.iff_dropout(None, 9, 4, None, 0, 0, None, 0, None, None), b"type 9")
     refused(L.iff_dropout(None, 0, -4, None, 0, 0, None, 0, None, None), b"bad size")
     refused(L.iff_dropout(None, 0, 4, None, 65537, 0, None, 0, None, None), b"threshold")
