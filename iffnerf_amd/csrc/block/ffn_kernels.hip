@@ -12,6 +12,12 @@
 
 #include <algorithm>
 
+#ifndef FFN_NB
+#define FFN_NB 2
+#endif
+#ifndef FFN_KT
+#define FFN_KT 64
+#endif
 namespace {
 
 enum { ACT_SILU = 0, ACT_GELU = 1 };
@@ -126,9 +132,9 @@ struct Prod {
     // EPI_OUT: out[row(m)][n] = acc + bias[n], ld N; row(m) = m, or with two halves of `half_pad` padded rows each, of which `half` exist.
     // With `part`: the fp32 share of a split over k instead, part[z][row][n] of rows_out rows
     void* out; const void* bias; float* part; int64_t half_pad, half, rows_out; bool vec_out;
-    // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld HP = pad8(H); factors p, q [M][HP] or null; bias b12
-    // EPI_DH: out = [dg | du] planes of ld 2 HP
-    int64_t up_row, HP; float* p; float* q; int act;
+    // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld ldo; factors p, q [M][HP = pad8(H)] or null; bias b12
+    // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
+    int64_t up_row, HP, ldo; float* p; float* q; int act;
 };
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
@@ -144,19 +150,21 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
     tn = t / rows;
 }
 
-// Tiles of 32 MR WM x 32 NR WN, 64 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
-// 1 KB per instruction, lane-linear in LDS) into two buffers: step t + 1 travels while step t is multiplied.  A KC tile is rows of 64 k
-// (128 B), its 16-byte chunk c in slot c ^ (row / 2 & 7); a KS tile is rows of one k (64 or 128 chunks of m), chunk c in slot
+// Tiles of 32 MR WM x 32 NR WN, 32 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
+// 1 KB per instruction, lane-linear in LDS) into a ring of NBUF buffers.  A KC tile is rows of 32 k
+// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k (64 or 128 chunks of m), chunk c in slot
 // c ^ 4 (k & 3), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
 // keep every LDS read free of bank conflicts.
-template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR>
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
     typedef typename Mat<T>::e E;
     typedef typename Vec8<E>::t E8;
     constexpr int P = Mat<T>::P, NW = WM * WN, BM = 32 * MR * WM, BN = 32 * NR * WN;
-    constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;                 // 1-KB pieces per wave and step
-    constexpr int TILE = (BM + BN) * 128;
-    __shared__ __attribute__((aligned(1024))) char s_all[2 * TILE];
+    constexpr int ROW = KT * 2, PA = BM * ROW / 1024 / NW, PB = BN * ROW / 1024 / NW;      // 1-KB pieces per wave and step
+    constexpr int TILE = (BM + BN) * ROW, GW = 16 * NR;
+    constexpr int OLD = 32 * NR + 4;                                  // floats per row of a wave's output tile in LDS: conflict-free 16-byte writes down a column
+    constexpr int POOL = NBUF * TILE > NW * 32 * OLD * 4 ? NBUF * TILE : NW * 32 * OLD * 4;
+    __shared__ __attribute__((aligned(1024))) char s_all[POOL];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, lh = lane >> 5;
     const int wm = (wave / WN) * 32 * MR, wn = (wave % WN) * 32 * NR;
     unsigned tm, tn;
@@ -167,31 +175,33 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigne
     const E* const A = reinterpret_cast<const E*>(g.a.p);
     const E* const B = reinterpret_cast<const E*>(g.b.p);
 
+    const auto swizzle = [](int r) { return KT == 64 ? (r >> 1) & 7 : (r >> 2) & 3; };
+
     // the lane's source of each piece, in bytes from the tile's corner at the step's k (ld < 2^22: 256 rows stay below 2^31), and its first k
     uint32_t oa[PA], ob[PB];
     int ka[PA], kb[PB];
 #pragma unroll
     for (int i = 0; i < PA; ++i) {
         const int at = (wave + NW * i) * 1024 + lane * 16;
-        const int r = at / (AK == KC ? 128 : BM * 2), c = ((at % (AK == KC ? 128 : BM * 2)) >> 4) ^ (AK == KC ? (r >> 1) & 7 : (r & 3) << 2);
+        const int r = at / (AK == KC ? ROW : BM * 2), c = ((at % (AK == KC ? ROW : BM * 2)) >> 4) ^ (AK == KC ? swizzle(r) : (r & 3) << 2);
         if (AK == KC) { oa[i] = (uint32_t)((min(m0 + r, g.ra - 1) - m0) * g.a.ld + c * 8) * 2; ka[i] = c * 8; }
         else { oa[i] = (uint32_t)(r * g.a.ld + min(m0 + c * 8, g.a.ld - 8) - m0) * 2; ka[i] = r; }
     }
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
         const int at = (wave + NW * i) * 1024 + lane * 16;
-        const int r = at / (BK == KC ? 128 : BN * 2), c = ((at % (BK == KC ? 128 : BN * 2)) >> 4) ^ (BK == KC ? (r >> 1) & 7 : (r & 3) << 2);
+        const int r = at / (BK == KC ? ROW : BN * 2), c = ((at % (BK == KC ? ROW : BN * 2)) >> 4) ^ (BK == KC ? swizzle(r) : (r & 3) << 2);
         if (BK == KC) {
-            // a gate tile's rows: 32 gate rows, the 32 up rows of the same hidden units, the next 32 gate rows ...
-            const int64_t row = EPI == EPI_GATE ? min(n0 + (r >> 6) * 32 + (r & 31), g.N - 1) : min(n0 + r, g.rb - 1);
+            // a gate tile's rows, per wave: GW gate rows, then the up rows of the same hidden units
+            const int64_t row = EPI == EPI_GATE ? min(n0 + r / (2 * GW) * GW + r % GW, g.N - 1) : min(n0 + r, g.rb - 1);
             ob[i] = (uint32_t)((row - n0) * g.b.ld + c * 8) * 2;
             kb[i] = c * 8;
         } else { ob[i] = (uint32_t)(r * g.b.ld + min(n0 + c * 8, g.b.ld - 8) - n0) * 2; kb[i] = r; }
     }
-    const int64_t sa = AK == KC ? 64 : 64 * g.a.ld, sb = BK == KC ? 64 : 64 * g.b.ld;            // elements per step
+    const int64_t sa = AK == KC ? KT : KT * g.a.ld, sb = BK == KC ? KT : KT * g.b.ld;            // elements per step
     const E* const a0 = A + (AK == KC ? m0 * g.a.ld + k_lo : k_lo * g.a.ld + m0);
     const E* const b0 = B + (BK == KC ? n0 * g.b.ld + k_lo : k_lo * g.b.ld + n0);
-    const int steps_k = (int)((k_hi - k_lo + 63) / 64), steps = k_hi > k_lo ? steps_k * (P == 3 ? 6 : 1) : 0;
+    const int steps_k = (int)((k_hi - k_lo + KT - 1) / KT), steps = k_hi > k_lo ? steps_k * (P == 3 ? 6 : 1) : 0;
 
     auto issue = [&](int pair, int kt, int buf) {
         // planes of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
@@ -199,31 +209,31 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigne
         const char* as = reinterpret_cast<const char*>(a0 + pa * g.a.plane + kt * sa);
         const char* bs = reinterpret_cast<const char*>(b0 + pb * g.b.plane + kt * sb);
         char* dst = s_all + buf * TILE + wave * 1024;
-        const int64_t left = k_hi - k_lo - (int64_t)kt * 64;          // k values from this step on
+        const int64_t left = k_hi - k_lo - (int64_t)kt * KT;          // k values from this step on
         const auto load = [&](const char* src, char* to) {
             __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
         };
-        const auto b_base = [&](int i) { return EPI == EPI_GATE && (((wave + NW * i) >> 2) & 1) ? bs + g.up_row * g.b.ld * 2 : bs; };
-        if (left >= 64) {
+        const auto b_base = [&](int i) { return EPI == EPI_GATE && (((wave + NW * i) * (1024 / ROW) / GW) & 1) ? bs + g.up_row * g.b.ld * 2 : bs; };
+        if (left >= KT) {
 #pragma unroll
             for (int i = 0; i < PA; ++i) load(as + oa[i], dst + i * NW * 1024);
 #pragma unroll
-            for (int i = 0; i < PB; ++i) load(b_base(i) + ob[i], dst + BM * 128 + i * NW * 1024);
+            for (int i = 0; i < PB; ++i) load(b_base(i) + ob[i], dst + BM * ROW + i * NW * 1024);
         } else {                                                      // the last, partly filled step: zeros behind k_hi
             const char* const zero = reinterpret_cast<const char*>(g_zeros);
 #pragma unroll
             for (int i = 0; i < PA; ++i) load(ka[i] < left ? as + oa[i] : zero, dst + i * NW * 1024);
 #pragma unroll
-            for (int i = 0; i < PB; ++i) load(kb[i] < left ? b_base(i) + ob[i] : zero, dst + BM * 128 + i * NW * 1024);
+            for (int i = 0; i < PB; ++i) load(kb[i] < left ? b_base(i) + ob[i] : zero, dst + BM * ROW + i * NW * 1024);
         }
     };
 
     // where this lane's fragments are in a tile: KC one 16-byte read per 16 k, KS two transposed 8-byte reads
-    constexpr int ROWA = AK == KC ? 128 : BM * 2, ROWB = BK == KC ? 128 : BN * 2;
-    const int sw = (lr >> 1) & 7, trow = 8 * lh + ((lane & 15) >> 2), tx = ((lane >> 2) & 3) << 2;
+    constexpr int ROWA = AK == KC ? ROW : BM * 2, ROWB = BK == KC ? ROW : BN * 2;
+    const int sw = swizzle(lr), trow = 8 * lh + ((lane & 15) >> 2), tx = ((lane >> 2) & 3) << 2;
     const int tcol = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
     auto frag = [&](const char* tile, int kind, int rowbytes, int base, int j, int ks) -> E8 {
-        if (kind == KC) return *reinterpret_cast<const E8*>(tile + (base + 32 * j + lr) * 128 + (((2 * ks + lh) ^ sw) << 4));
+        if (kind == KC) return *reinterpret_cast<const E8*>(tile + (base + 32 * j + lr) * ROW + (((2 * ks + lh) ^ sw) << 4));
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         const char* at = tile + (16 * ks + trow) * rowbytes + (((base / 8 + 4 * j) ^ tx) << 4) + tcol;
@@ -240,106 +250,168 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigne
         for (int m = 0; m < MR; ++m)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[n][m][r] = 0.0f;
-    int pair = 0, kt = 0;
-    if (steps) issue(0, 0, 0);
-    for (int t = 0; t < steps; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // this wave's pieces of step t have landed ...
-        __builtin_amdgcn_s_barrier();                                 // ... everybody's have, and everybody has read step t - 1
-        asm volatile("" ::: "memory");
-        if (++kt == steps_k) { kt = 0; ++pair; }
-        if (t + 1 < steps) issue(pair, kt, (t + 1) & 1);
-        const char* const ta = s_all + (t & 1) * TILE;
-        const char* const tb = ta + BM * 128;
+    // A ring of NBUF buffers.  A step is two blocks of 16 k; while block b is multiplied the fragments of block b + 1 are read, across the
+    // step's border too: half way through step t everybody's pieces of step t + 1 have landed (a counted wait -- a __syncthreads would drain
+    // the queue -- and the barrier) and step t has been read by everybody, so step t + NBUF is requested into its buffer
+    struct Frags { E8 a[MR], b[NR]; };
+    const auto read = [&](Frags& f, int buf, int ks) {
+        const char* const ta = s_all + buf * TILE;
+        const char* const tb = ta + BM * ROW;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            E8 fa[MR], fb[NR];
+        for (int j = 0; j < NR; ++j) f.b[j] = frag(tb, BK, ROWB, wn, j, ks);
 #pragma unroll
-            for (int j = 0; j < NR; ++j) fb[j] = frag(tb, BK, ROWB, wn, j, ks);
+        for (int j = 0; j < MR; ++j) f.a[j] = frag(ta, AK, ROWA, wm, j, ks);
+    };
+    const auto multiply = [&](const Frags& f) {
 #pragma unroll
-            for (int j = 0; j < MR; ++j) fa[j] = frag(ta, AK, ROWA, wm, j, ks);
+        for (int m = 0; m < MR; ++m)
 #pragma unroll
-            for (int m = 0; m < MR; ++m)
+            for (int n = 0; n < NR; ++n) acc[n][m] = mfma(f.b[n], f.a[m], acc[n][m]);
+    };
+    // 0x100: LDS reads, 0x8: matrix instructions -- the reads go out between the first products
+    const auto interleave = [&]() {
+        constexpr int READS = MR * (AK == KC ? 1 : 2) + NR * (BK == KC ? 1 : 2), PER = (READS + MR * NR - 2) / (MR * NR - 1);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[n][m] = mfma(fb[n], fa[m], acc[n][m]);
+        for (int i = 0; i < MR * NR - 1; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto landed = [&](int younger) {                            // all but the `younger` last requested steps of this wave
+        if (younger >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * (PA + PB)) : "memory");
+        else if (younger == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (PA + PB)) : "memory");
+        else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PA + PB) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    int pair = 0, kt = 0, head = 0, cur = 0;
+    const auto request = [&]() {
+        issue(pair, kt, head);
+        if (++kt == steps_k) { kt = 0; ++pair; }
+        head = head + 1 == NBUF ? 0 : head + 1;
+    };
+    Frags f0, f1;
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i)
+        if (i < steps) request();
+    if (steps) {
+        landed(min(NBUF, steps) - 1);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(f0, 0, 0);
+    }
+    for (int t = 0; t < steps; ++t) {
+#pragma unroll
+        for (int ks = 0; ks < KT / 16 - 1; ++ks) {
+            read(ks & 1 ? f0 : f1, cur, ks + 1);
+            multiply(ks & 1 ? f1 : f0);
+            interleave();
+        }
+        const int nxt = cur + 1 == NBUF ? 0 : cur + 1;
+        if (t + 1 < steps) {
+            landed(min(NBUF - 2, steps - 2 - t));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (t + NBUF < steps) request();
+            __builtin_amdgcn_sched_barrier(0);
+            read(f0, nxt, 0);
+        }
+        multiply(f1);
+        interleave();
+        cur = nxt;
     }
 
-    // a lane holds row m = lr of C and columns (reg & 3) + 8 (reg >> 2) + 4 lh of each 32 x 32 block
+    // A lane holds row m = lr of C and columns (reg & 3) + 8 (reg >> 2) + 4 lh of each 32 x 32 block: stored from there an instruction
+    // touches 32 rows with 16 bytes each.  Every wave turns its 32-row slices over in LDS instead and works along the rows, 4 columns per lane:
+    // whole 128- to 512-byte runs (the direct form cost 76 us of F2's 271, 371 of the gate product's 735 at 16448 x 1536 x 4096)
     const T* const bias = reinterpret_cast<const T*>(g.bias);
+    float* const tile = reinterpret_cast<float*>(s_all) + wave * 32 * OLD;
+    constexpr int CPL = EPI == EPI_GATE ? GW / 4 : 8 * NR, RPI = 64 / CPL;          // lanes per row, rows per pass
+    const int col = (lane % CPL) * 4;
+    const int64_t n = n0 + (EPI == EPI_GATE ? wn / 2 : wn) + col;
+    float bi[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool in = bias && n + i < g.N;
+        bi[0][i] = in ? (float)bias[n + i] : 0.0f;
+        bi[1][i] = in && EPI == EPI_GATE ? (float)bias[g.N + n + i] : 0.0f;
+    }
+    __syncthreads();                                                  // everybody has read the last fragments
 #pragma unroll
     for (int mb = 0; mb < MR; ++mb) {
-        const int64_t m = m0 + wm + 32 * mb + lr;
-        if (m >= g.M) continue;
-        if constexpr (EPI == EPI_GATE) {
-            static_assert(NR == 2, "a wave's columns are 32 gate and 32 up columns");
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const int64_t n = n0 + (wn >> 1) + 8 * q4 + 4 * lh;
+        for (int nb = 0; nb < NR; ++nb)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4*>(tile + lr * OLD + 32 * nb + 8 * q4 + 4 * lh) =
+                    f32x4{acc[nb][mb][4 * q4], acc[nb][mb][4 * q4 + 1], acc[nb][mb][4 * q4 + 2], acc[nb][mb][4 * q4 + 3]};
+#pragma unroll
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int r = it * RPI + lane / CPL;
+            const int64_t m = m0 + wm + 32 * mb + r;
+            float v[4];
+            Pack<float, 4>::load(tile + r * OLD + col, v);
+            if (m >= g.M) continue;
+            if constexpr (EPI == EPI_GATE) {
                 if (n >= g.HP) continue;
-                float hv[4], pv[4], qv[4];
+                float u[4], hv[4], pv[4];
+                Pack<float, 4>::load(tile + r * OLD + GW + col, u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const bool in = n + i < g.N;
-                    const float gv = acc[0][mb][4 * q4 + i] + (in && bias ? (float)bias[n + i] : 0.0f);
-                    const float uv = acc[1][mb][4 * q4 + i] + (in && bias ? (float)bias[g.N + n + i] : 0.0f);
+                    const float gv = v[i] + bi[0][i], uv = u[i] + bi[1][i];
                     float f, df;
                     activation<P == 3>(g.act, gv, f, df);
                     hv[i] = in ? f * uv : 0.0f;
                     pv[i] = in ? uv * df : 0.0f;
-                    qv[i] = in ? f : 0.0f;
+                    v[i] = in ? f : 0.0f;
                 }
-                store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.HP + n, g.M * g.HP, hv);
+                store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.M * g.ldo, hv);
                 if (g.p) {
                     Pack<float, 4>::store(g.p + m * g.HP + n, pv);
-                    Pack<float, 4>::store(g.q + m * g.HP + n, qv);
+                    Pack<float, 4>::store(g.q + m * g.HP + n, v);
                 }
-            }
-        } else {
-            int64_t row = m;
-            if (EPI == EPI_OUT && g.half_pad) {
-                const int64_t hf = m >= g.half_pad;
-                if (m - hf * g.half_pad >= g.half) continue;
-                row = hf * g.half + m - hf * g.half_pad;
-            }
+            } else if constexpr (EPI == EPI_DH) {
+                if (n >= g.HP) continue;
+                float p[4], q[4];
+                Pack<float, 4>::load(g.p + m * g.HP + n, p);
+                Pack<float, 4>::load(g.q + m * g.HP + n, q);
 #pragma unroll
-            for (int nb = 0; nb < NR; ++nb)
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const int64_t n = n0 + wn + 32 * nb + 8 * q4 + 4 * lh;
-                    float v[4] = {acc[nb][mb][4 * q4], acc[nb][mb][4 * q4 + 1], acc[nb][mb][4 * q4 + 2], acc[nb][mb][4 * q4 + 3]};
-                    if constexpr (EPI == EPI_DH) {
-                        if (n >= g.HP) continue;
-                        float p[4], q[4];
-                        Pack<float, 4>::load(g.p + m * g.HP + n, p);
-                        Pack<float, 4>::load(g.q + m * g.HP + n, q);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool in = n + i < g.N;
-                            p[i] = in ? v[i] * p[i] : 0.0f;
-                            q[i] = in ? v[i] * q[i] : 0.0f;
-                        }
-                        E* o = reinterpret_cast<E*>(g.out) + m * 2 * g.HP + n;
-                        store_planes<T>(o, g.M * 2 * g.HP, p);
-                        store_planes<T>(o + g.HP, g.M * 2 * g.HP, q);
-                    } else if (g.part) {
-                        float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
-                        if (g.vec_out && n < g.N) Pack<float, 4>::store(o, v);
-                        else
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (n + i < g.N) o[i] = v[i];
-                    } else {
-                        T* o = reinterpret_cast<T*>(g.out) + row * g.N + n;
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = n + i < g.N;
+                    p[i] = in ? v[i] * p[i] : 0.0f;
+                    q[i] = in ? v[i] * q[i] : 0.0f;
+                }
+                E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
+                store_planes<T>(o, g.M * g.ldo, p);
+                store_planes<T>(o + g.HP, g.M * g.ldo, q);
+            } else {
+                int64_t row = m;
+                if (g.half_pad) {
+                    const int64_t hf = m >= g.half_pad;
+                    if (m - hf * g.half_pad >= g.half) continue;
+                    row = hf * g.half + m - hf * g.half_pad;
+                }
+                if (g.part) {
+                    float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
+                    if (g.vec_out && n < g.N) Pack<float, 4>::store(o, v);
+                    else
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (bias && n + i < g.N) v[i] += (float)bias[n + i];
-                        if (g.vec_out && n < g.N) store4<T>(o, v);
-                        else
+                            if (n + i < g.N) o[i] = v[i];
+                } else {
+                    T* o = reinterpret_cast<T*>(g.out) + row * g.N + n;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (n + i < g.N) o[i] = (T)v[i];
-                    }
+                    for (int i = 0; i < 4; ++i) v[i] += bi[0][i];
+                    if (g.vec_out && n < g.N) store4<T>(o, v);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (n + i < g.N) o[i] = (T)v[i];
                 }
+            }
         }
     }
 }
@@ -403,14 +475,14 @@ hipError_t operand(Work& w, const void* src, int64_t halves, int64_t R, int64_t 
     return hipGetLastError();
 }
 
-template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR>
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
 hipError_t tiles(Prod g, int splits, hipStream_t s) {
     constexpr int BM = 32 * MR * WM, NT = EPI == EPI_GATE ? 16 * NR * WN : 32 * NR * WN;
     const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M + BM - 1) / BM, gn = (N + NT - 1) / NT;
     if (!gm || !gn) return hipSuccess;
     if (gm * gn > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 63) / 64 * 64 : std::max<int64_t>(g.K, 64);
-    k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
+    k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, KT, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
     return hipGetLastError();
 }
 inline int64_t tile_count(int64_t M, int64_t N, int side) { return ((M + side - 1) / side) * ((N + side - 1) / side); }
@@ -419,8 +491,8 @@ inline int64_t tile_count(int64_t M, int64_t N, int side) { return ((M + side - 
 template <class T, int AK, int BK, int EPI>
 hipError_t product(const Prod& g, int splits, hipStream_t s) {
     const int64_t N = EPI == EPI_GATE ? 2 * g.HP : EPI == EPI_DH ? g.HP : g.N;
-    if (tile_count(g.M, N, 256) * splits >= 192) return tiles<T, AK, BK, EPI, 2, 4, 4, 2>(g, splits, s);
-    return tiles<T, AK, BK, EPI, 2, 2, 2, 2>(g, splits, s);
+    if (tile_count(g.M, N, 256) * splits >= 192) return tiles<T, AK, BK, EPI, 4, 2, 2, 4, FFN_KT, FFN_NB>(g, splits, s);
+    return tiles<T, AK, BK, EPI, 2, 2, 2, 2, FFN_KT, FFN_NB>(g, splits, s);
 }
 
 // shares of a weight gradient's sum over the rows, when its tiles alone do not fill the chip: each at least 512 deep
@@ -464,7 +536,7 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
     if (w.counting()) return hipSuccess;
     Prod g{};
-    g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.up_row = HP;
+    g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
     FFN_TRY((product<T, KC, KC, EPI_GATE>(g, 1, w.s)));
     Prod d{};
@@ -483,13 +555,14 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     const float* p = (const float*)(h + (all ? 0 : kept_h<T>(f.M, f.H)));
     Operand dy{};
     if (hidden || f.dw3) FFN_TRY(operand<T>(w, f.dy, 1, f.M, f.O, dy));
-    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
+    const int64_t GL = 2 * HP;
+    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, GL)) : nullptr, GL, f.M * GL};
     if (hidden) {
         Operand w3;
         FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
         if (!all) {
             Prod g{};
-            g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP;
+            g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = GL;
             g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
             FFN_TRY((product<T, KC, KS, EPI_DH>(g, 1, w.s)));
         }
@@ -515,7 +588,7 @@ hipError_t backward(const FfnArgs& f, Work& w) {
         g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
         FFN_TRY(weight_gradient<T>(w, g, f.O));
     }
-    if (all || f.db12) FFN_TRY((colsum<T, E, P>(w, dgu.p, 2 * HP, dgu.plane, f.M, 2 * (int64_t)f.H, HP, f.H, f.db12)));
+    if (all || f.db12) FFN_TRY((colsum<T, E, P>(w, dgu.p, GL, dgu.plane, f.M, 2 * (int64_t)f.H, HP, f.H, f.db12)));
     if (all || f.db3) FFN_TRY((colsum<T, T, 1>(w, f.dy, f.O, 0, f.M, f.O, 0, 0, f.db3)));
     return hipSuccess;
 }
