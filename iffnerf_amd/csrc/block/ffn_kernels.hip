@@ -11,9 +11,13 @@
 #include "block_types.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #ifndef FFN_NB
 #define FFN_NB 2
+#endif
+#ifndef FFN_BIG
+#define FFN_BIG 4, 2, 2, 4
 #endif
 #ifndef FFN_KT
 #define FFN_KT 64
@@ -134,7 +138,8 @@ struct Prod {
     void* out; const void* bias; float* part; int64_t half_pad, half, rows_out; bool vec_out;
     // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld ldo; factors p, q [M][HP = pad8(H)] or null; bias b12
     // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
-    int64_t up_row, HP, ldo; float* p; float* q; int act;
+    // and with `sums`: [m slice][2H] column sums of dg and du (fp32, before they are rounded) over the slice's 32 MR rows
+    int64_t up_row, HP, ldo; float* p; float* q; int act; float* sums;
 };
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
@@ -156,7 +161,7 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
 // c ^ 4 (k & 3), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
 // keep every LDS read free of bank conflicts.
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
+__global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
     typedef typename Mat<T>::e E;
     typedef typename Vec8<E>::t E8;
     constexpr int P = Mat<T>::P, NW = WM * WN, BM = 32 * MR * WM, BN = 32 * NR * WN;
@@ -338,6 +343,77 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigne
         bi[0][i] = in ? (float)bias[n + i] : 0.0f;
         bi[1][i] = in && EPI == EPI_GATE ? (float)bias[g.N + n + i] : 0.0f;
     }
+    float sg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool whole = m0 + BM <= g.M && n0 + NT <= g.N && !g.half_pad && (EPI != EPI_OUT || g.vec_out);
+    const auto slice = [&](int mb, int it, auto all_inside) {
+        constexpr bool IN = decltype(all_inside)::value;
+        const int r = it * RPI + lane / CPL;
+        const int64_t m = m0 + wm + 32 * mb + r;
+        float v[4];
+        Pack<float, 4>::load(tile + r * OLD + col, v);
+        if (!IN && m >= g.M) return;
+        if constexpr (EPI == EPI_GATE) {
+            if (!IN && n >= g.HP) return;
+            float u[4], hv[4], pv[4];
+            Pack<float, 4>::load(tile + r * OLD + GW + col, u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = IN || n + i < g.N;
+                const float gv = v[i] + bi[0][i], uv = u[i] + bi[1][i];
+                float f, df;
+                activation<P == 3>(g.act, gv, f, df);
+                hv[i] = in ? f * uv : 0.0f;
+                pv[i] = in ? uv * df : 0.0f;
+                v[i] = in ? f : 0.0f;
+            }
+            store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.M * g.ldo, hv);
+            if (g.p) {
+                Pack<float, 4>::store(g.p + m * g.HP + n, pv);
+                Pack<float, 4>::store(g.q + m * g.HP + n, v);
+            }
+        } else if constexpr (EPI == EPI_DH) {
+            if (!IN && n >= g.HP) return;
+            float p[4], q[4];
+            Pack<float, 4>::load(g.p + m * g.HP + n, p);
+            Pack<float, 4>::load(g.q + m * g.HP + n, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = IN || n + i < g.N;
+                p[i] = in ? v[i] * p[i] : 0.0f;
+                q[i] = in ? v[i] * q[i] : 0.0f;
+                sg[i] += p[i];
+                su[i] += q[i];
+            }
+            E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
+            store_planes<T>(o, g.M * g.ldo, p);
+            store_planes<T>(o + g.HP, g.M * g.ldo, q);
+        } else {
+            int64_t row = m;
+            if (!IN && g.half_pad) {
+                const int64_t hf = m >= g.half_pad;
+                if (m - hf * g.half_pad >= g.half) return;
+                row = hf * g.half + m - hf * g.half_pad;
+            }
+            const bool vec = IN || (g.vec_out && n < g.N);
+            if (g.part) {
+                float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
+                if (vec) Pack<float, 4>::store(o, v);
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < g.N) o[i] = v[i];
+            } else {
+                T* o = reinterpret_cast<T*>(g.out) + row * g.N + n;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += bi[0][i];
+                if (vec) store4<T>(o, v);
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < g.N) o[i] = (T)v[i];
+            }
+        }
+    };
     __syncthreads();                                                  // everybody has read the last fragments
 #pragma unroll
     for (int mb = 0; mb < MR; ++mb) {
@@ -347,70 +423,25 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_ffn_product(Prod g, unsigne
             for (int q4 = 0; q4 < 4; ++q4)
                 *reinterpret_cast<f32x4*>(tile + lr * OLD + 32 * nb + 8 * q4 + 4 * lh) =
                     f32x4{acc[nb][mb][4 * q4], acc[nb][mb][4 * q4 + 1], acc[nb][mb][4 * q4 + 2], acc[nb][mb][4 * q4 + 3]};
+        // a tile that lies wholly inside C: no checks between the passes, so that their reads and stores overlap
+        if (whole) {
 #pragma unroll
-        for (int it = 0; it < 32 / RPI; ++it) {
-            const int r = it * RPI + lane / CPL;
-            const int64_t m = m0 + wm + 32 * mb + r;
-            float v[4];
-            Pack<float, 4>::load(tile + r * OLD + col, v);
-            if (m >= g.M) continue;
-            if constexpr (EPI == EPI_GATE) {
-                if (n >= g.HP) continue;
-                float u[4], hv[4], pv[4];
-                Pack<float, 4>::load(tile + r * OLD + GW + col, u);
+            for (int it = 0; it < 32 / RPI; ++it) slice(mb, it, std::true_type{});
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = n + i < g.N;
-                    const float gv = v[i] + bi[0][i], uv = u[i] + bi[1][i];
-                    float f, df;
-                    activation<P == 3>(g.act, gv, f, df);
-                    hv[i] = in ? f * uv : 0.0f;
-                    pv[i] = in ? uv * df : 0.0f;
-                    v[i] = in ? f : 0.0f;
-                }
-                store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.M * g.ldo, hv);
-                if (g.p) {
-                    Pack<float, 4>::store(g.p + m * g.HP + n, pv);
-                    Pack<float, 4>::store(g.q + m * g.HP + n, v);
-                }
-            } else if constexpr (EPI == EPI_DH) {
-                if (n >= g.HP) continue;
-                float p[4], q[4];
-                Pack<float, 4>::load(g.p + m * g.HP + n, p);
-                Pack<float, 4>::load(g.q + m * g.HP + n, q);
+            for (int it = 0; it < 32 / RPI; ++it) slice(mb, it, std::false_type{});
+        }
+    }
+    if constexpr (EPI == EPI_DH) {
+        if (!g.sums) return;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = n + i < g.N;
-                    p[i] = in ? v[i] * p[i] : 0.0f;
-                    q[i] = in ? v[i] * q[i] : 0.0f;
-                }
-                E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
-                store_planes<T>(o, g.M * g.ldo, p);
-                store_planes<T>(o + g.HP, g.M * g.ldo, q);
-            } else {
-                int64_t row = m;
-                if (g.half_pad) {
-                    const int64_t hf = m >= g.half_pad;
-                    if (m - hf * g.half_pad >= g.half) continue;
-                    row = hf * g.half + m - hf * g.half_pad;
-                }
-                if (g.part) {
-                    float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
-                    if (g.vec_out && n < g.N) Pack<float, 4>::store(o, v);
-                    else
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (n + i < g.N) o[i] = v[i];
-                } else {
-                    T* o = reinterpret_cast<T*>(g.out) + row * g.N + n;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += bi[0][i];
-                    if (g.vec_out && n < g.N) store4<T>(o, v);
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (n + i < g.N) o[i] = (T)v[i];
-                }
+            for (int off = CPL; off < 64; off <<= 1) { sg[i] += __shfl_xor(sg[i], off, 64); su[i] += __shfl_xor(su[i], off, 64); }
+            if (lane < CPL && n + i < g.N) {
+                float* o = g.sums + ((int64_t)tm * WM + wave / WN) * 2 * g.N + n + i;
+                o[0] = sg[i];
+                o[g.N] = su[i];
             }
         }
     }
@@ -426,23 +457,52 @@ __global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part
     }
 }
 
-// column sums of [M][ld] planes over the rows y, y + gridDim.y, ...: part[y][column]; with halves of half_pad padded columns the pads are
-// left out.  k_ffn_join adds the shares
-template <class S, int P>
-__global__ void __launch_bounds__(256) k_ffn_colsum(const S* __restrict__ a, int64_t ld, int64_t plane, int64_t M, int64_t N, int64_t half_pad,
-                                                    int64_t half, float* __restrict__ part) {
-    const int64_t n = blockIdx.x * (int64_t)256 + threadIdx.x;
-    if (n >= N) return;
-    const int64_t c = half_pad && n >= half ? n - half + half_pad : n;
-    float v = 0.0f;
-    for (int64_t m = blockIdx.y; m < M; m += gridDim.y)
+// out[c] = sum_g part[g][c]: 16 columns x 16 groups of shares per workgroup, groups joined in order
+template <class T>
+__global__ void __launch_bounds__(256) k_ffn_join_columns(const float* __restrict__ part, int64_t G, int64_t N, T* __restrict__ out) {
+    __shared__ float s[16][17];
+    const int c16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
+    const int64_t c = blockIdx.x * (int64_t)16 + c16;
+    float a = 0.0f;
+    if (c < N)
+#pragma unroll 8
+        for (int64_t g = grp; g < G; g += 16) a += part[g * N + c];
+    s[grp][c16] = a;
+    __syncthreads();
+    if (grp == 0 && c < N) {
+        for (int j = 1; j < 16; ++j) a += s[j][c16];
+        out[c] = (T)a;
+    }
+}
+
+// shares of the column sums of a [M][N] matrix: part[y][n] over the rows of block y (every gridDim.y-th group of 8); V columns per thread
+template <class T, int V>
+__global__ void __launch_bounds__(256) k_ffn_colsum(const T* __restrict__ a, int64_t M, int64_t N, float* __restrict__ part) {
+    __shared__ float s[8][32 * V + 1];
+    const int c = (threadIdx.x & 31) * V, r8 = threadIdx.x >> 5;
+    const int64_t n = blockIdx.x * (int64_t)(32 * V) + c;
+    float v[V];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p) v += (float)a[p * plane + m * ld + c];
-    part[blockIdx.y * N + n] = v;
+    for (int i = 0; i < V; ++i) v[i] = 0.0f;
+    if (n < N)
+#pragma unroll 4
+        for (int64_t m = blockIdx.y * (int64_t)8 + r8; m < M; m += (int64_t)gridDim.y * 8) {
+            float t[V];
+            Pack<T, V>::load(a + m * N + n, t);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] += t[i];
+        }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[r8][c + i] = v[i];
+    __syncthreads();
+    for (int j = threadIdx.x; j < 32 * V; j += 256) {
+        float t = s[0][j];
+        for (int r = 1; r < 8; ++r) t += s[r][j];
+        if (blockIdx.x * (int64_t)(32 * V) + j < N) part[blockIdx.y * N + blockIdx.x * (int64_t)(32 * V) + j] = t;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-constexpr int CSUM = 64;                                         // shares of a column sum
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -487,11 +547,19 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
 }
 inline int64_t tile_count(int64_t M, int64_t N, int side) { return ((M + side - 1) / side) * ((N + side - 1) / side); }
 
-// 256 x 256 tiles (8 waves) where they fill the chip, else 128 x 128 (4 waves)
+// 256 x 256 tiles (8 waves of 64 x 128) where they fill the chip, else 128 x 128 (4 waves of 64 x 64)
+template <int EPI>
+inline bool big_tiles(const Prod& g, int splits) {
+    const int64_t N = EPI == EPI_GATE ? 2 * g.HP : EPI == EPI_DH ? g.HP : g.N;
+    return tile_count(g.M, N, 256) * splits >= 192;
+}
+// the 64-row slices whose column sums EPI_DH leaves
+template <int EPI>
+inline int64_t row_slices(const Prod& g) { return big_tiles<EPI>(g, 1) ? (g.M + 255) / 256 * 4 : (g.M + 127) / 128 * 2; }
+
 template <class T, int AK, int BK, int EPI>
 hipError_t product(const Prod& g, int splits, hipStream_t s) {
-    const int64_t N = EPI == EPI_GATE ? 2 * g.HP : EPI == EPI_DH ? g.HP : g.N;
-    if (tile_count(g.M, N, 256) * splits >= 192) return tiles<T, AK, BK, EPI, 4, 2, 2, 4, FFN_KT, FFN_NB>(g, splits, s);
+    if (big_tiles<EPI>(g, splits)) return tiles<T, AK, BK, EPI, FFN_BIG, FFN_KT, FFN_NB>(g, splits, s);
     return tiles<T, AK, BK, EPI, 2, 2, 2, 2, FFN_KT, FFN_NB>(g, splits, s);
 }
 
@@ -513,13 +581,23 @@ hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
     k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, w.s>>>(g.part, z, n, (T*)g.out);
     return hipGetLastError();
 }
-template <class T, class S, int P>
-hipError_t colsum(Work& w, const void* a, int64_t ld, int64_t plane, int64_t M, int64_t N, int64_t half_pad, int64_t half, void* out) {
-    float* part = (float*)w.take((size_t)CSUM * N * 4);
-    if (w.counting()) return hipSuccess;
-    k_ffn_colsum<S, P><<<dim3((unsigned)((N + 255) / 256), CSUM), 256, 0, w.s>>>((const S*)a, ld, plane, M, N, half_pad, half, part);
-    k_ffn_join<T><<<(unsigned)((N + 255) / 256), 256, 0, w.s>>>(part, CSUM, N, (T*)out);
+template <class T>
+hipError_t join_columns(const float* part, int64_t G, int64_t N, void* out, hipStream_t s) {
+    k_ffn_join_columns<T><<<(unsigned)((N + 15) / 16), 256, 0, s>>>(part, G, N, (T*)out);
     return hipGetLastError();
+}
+// shares: enough workgroups for the chip, each at least 64 rows
+template <class T>
+hipError_t colsum(Work& w, const void* a, int64_t M, int64_t N, void* out) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, 128));
+    float* part = (float*)w.take((size_t)shares * N * 4);
+    if (w.counting()) return hipSuccess;
+    if (N % V == 0 && aligned16(a))
+        k_ffn_colsum<T, V><<<dim3((unsigned)((N + 32 * V - 1) / (32 * V)), (unsigned)shares), 256, 0, w.s>>>((const T*)a, M, N, part);
+    else
+        k_ffn_colsum<T, 1><<<dim3((unsigned)((N + 31) / 32), (unsigned)shares), 256, 0, w.s>>>((const T*)a, M, N, part);
+    return join_columns<T>(part, shares, N, out, w.s);
 }
 
 // what the forward pass keeps: h planes, then p and q
@@ -547,8 +625,6 @@ hipError_t forward(const FfnArgs& f, Work& w) {
 
 template <class T>
 hipError_t backward(const FfnArgs& f, Work& w) {
-    typedef typename Mat<T>::e E;
-    constexpr int P = Mat<T>::P;
     const int64_t HP = pad8(f.H);
     const bool all = w.counting(), hidden = all || f.dx || f.dw12 || f.db12;
     char* h = (char*)f.kept;
@@ -560,11 +636,15 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     if (hidden) {
         Operand w3;
         FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
+        const int64_t slices = (f.M + 127) / 128 * 4;                 // at most: row slices of 32 rows and more
+        float* sums = all || f.db12 ? (float*)w.take((size_t)slices * 2 * f.H * 4) : nullptr;
         if (!all) {
             Prod g{};
             g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = GL;
             g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
+            g.sums = sums;
             FFN_TRY((product<T, KC, KS, EPI_DH>(g, 1, w.s)));
+            if (f.db12) FFN_TRY(join_columns<T>(sums, row_slices<EPI_DH>(g), 2 * (int64_t)f.H, f.db12, w.s));
         }
     }
     if (all || f.dx) {
@@ -588,8 +668,7 @@ hipError_t backward(const FfnArgs& f, Work& w) {
         g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
         FFN_TRY(weight_gradient<T>(w, g, f.O));
     }
-    if (all || f.db12) FFN_TRY((colsum<T, E, P>(w, dgu.p, GL, dgu.plane, f.M, 2 * (int64_t)f.H, HP, f.H, f.db12)));
-    if (all || f.db3) FFN_TRY((colsum<T, T, 1>(w, f.dy, f.O, 0, f.M, f.O, 0, 0, f.db3)));
+    if (all || f.db3) FFN_TRY(colsum<T>(w, f.dy, f.M, f.O, f.db3));
     return hipSuccess;
 }
 
