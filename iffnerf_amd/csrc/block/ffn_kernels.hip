@@ -13,15 +13,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#ifndef FFN_NB
-#define FFN_NB 2
-#endif
-#ifndef FFN_BIG
-#define FFN_BIG 4, 2, 2, 4
-#endif
-#ifndef FFN_KT
-#define FFN_KT 64
-#endif
 namespace {
 
 enum { ACT_SILU = 0, ACT_GELU = 1 };
@@ -132,17 +123,24 @@ enum { EPI_OUT = 0, EPI_GATE = 1, EPI_DH = 2 };
 struct Prod {
     Operand a, b;
     int64_t ra, rb;                       // rows of a KC operand (reads are clamped to them)
-    int64_t M, N, K, k_per_split;
+    int64_t M, N, K, k_per_split, m_base;      // a launch covers the rows m_base .. M - 1 of C
     // EPI_OUT: out[row(m)][n] = acc + bias[n], ld N; row(m) = m, or with two halves of `half_pad` padded rows each, of which `half` exist.
     // With `part`: the fp32 share of a split over k instead, part[z][row][n] of rows_out rows
     void* out; const void* bias; float* part; int64_t half_pad, half, rows_out; bool vec_out;
     // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld ldo; factors p, q [M][HP = pad8(H)] or null; bias b12
     // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
-    // and with `sums`: [m slice][2H] column sums of dg and du (fp32, before they are rounded) over the slice's 32 MR rows
+    // and with `sums`: [M / 64][2H] column sums of dg and du (fp32, before they are rounded) over 64 rows each
     int64_t up_row, HP, ldo; float* p; float* q; int act; float* sums;
 };
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
+
+// 16 bytes per lane from `src` to LDS, lane-linear from byte `lds` on.  As assembly: behind the builtin the compiler drains the memory queue
+// before every transposed LDS read (it takes the two for aliases), which serialised the products with a k-strided operand (dW12 at
+// 16448 x 1536 x 4096: 745 against 497 us).  Nothing is returned to a register; the waits are the kernel's own counted ones.
+__device__ __forceinline__ void dma16(const char* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");      // (nothing else in these kernels uses m0)
+}
 
 // Workgroups are dealt round-robin over the 8 XCDs, each with its own L2.  The ones that share an XCD (ids equal mod 8) take a contiguous
 // range of tiles, and that range runs down columns of 8 tiles of m before it moves on in n: what is in flight on an XCD shares operands.
@@ -170,12 +168,13 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
     constexpr int OLD = 32 * NR + 4;                                  // floats per row of a wave's output tile in LDS: conflict-free 16-byte writes down a column
     constexpr int POOL = NBUF * TILE > NW * 32 * OLD * 4 ? NBUF * TILE : NW * 32 * OLD * 4;
     __shared__ __attribute__((aligned(1024))) char s_all[POOL];
+    const uint32_t s_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_all;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, lh = lane >> 5;
     const int wm = (wave / WN) * 32 * MR, wn = (wave % WN) * 32 * NR;
     unsigned tm, tn;
     tile_of(blockIdx.x, gm, gn, tm, tn);
     constexpr int NT = EPI == EPI_GATE ? BN / 2 : BN;                 // columns of C per tile (a gate tile: as many gate as up columns)
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * NT;
+    const int64_t m0 = g.m_base + (int64_t)tm * BM, n0 = (int64_t)tn * NT;
     const int64_t k_lo = blockIdx.y * g.k_per_split, k_hi = min(g.K, k_lo + g.k_per_split);
     const E* const A = reinterpret_cast<const E*>(g.a.p);
     const E* const B = reinterpret_cast<const E*>(g.b.p);
@@ -208,28 +207,34 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
     const E* const b0 = B + (BK == KC ? n0 * g.b.ld + k_lo : k_lo * g.b.ld + n0);
     const int steps_k = (int)((k_hi - k_lo + KT - 1) / KT), steps = k_hi > k_lo ? steps_k * (P == 3 ? 6 : 1) : 0;
 
-    auto issue = [&](int pair, int kt, int buf) {
-        // planes of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+    // the next step to request: planes of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); k values from it on.  Behind the
+    // last step `left` is not positive and the pieces are zeros: the queue holds the same number of pieces at every step
+    const char* as = reinterpret_cast<const char*>(a0);
+    const char* bs = reinterpret_cast<const char*>(b0);
+    int pair = 0, kt = 0, head = 0;
+    int left = steps ? (int)(k_hi - k_lo) : 0;
+    const auto planes = [&]() {
         const int pa = P == 1 ? 0 : pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = P == 1 ? 0 : pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
-        const char* as = reinterpret_cast<const char*>(a0 + pa * g.a.plane + kt * sa);
-        const char* bs = reinterpret_cast<const char*>(b0 + pb * g.b.plane + kt * sb);
-        char* dst = s_all + buf * TILE + wave * 1024;
-        const int64_t left = k_hi - k_lo - (int64_t)kt * KT;          // k values from this step on
-        const auto load = [&](const char* src, char* to) {
-            __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-        };
-        const auto b_base = [&](int i) { return EPI == EPI_GATE && (((wave + NW * i) * (1024 / ROW) / GW) & 1) ? bs + g.up_row * g.b.ld * 2 : bs; };
-        if (left >= KT) {
-#pragma unroll
-            for (int i = 0; i < PA; ++i) load(as + oa[i], dst + i * NW * 1024);
-#pragma unroll
-            for (int i = 0; i < PB; ++i) load(b_base(i) + ob[i], dst + BM * ROW + i * NW * 1024);
-        } else {                                                      // the last, partly filled step: zeros behind k_hi
-            const char* const zero = reinterpret_cast<const char*>(g_zeros);
-#pragma unroll
-            for (int i = 0; i < PA; ++i) load(ka[i] < left ? as + oa[i] : zero, dst + i * NW * 1024);
-#pragma unroll
-            for (int i = 0; i < PB; ++i) load(kb[i] < left ? b_base(i) + ob[i] : zero, dst + BM * ROW + i * NW * 1024);
+        as = reinterpret_cast<const char*>(a0 + pa * g.a.plane);
+        bs = reinterpret_cast<const char*>(b0 + pb * g.b.plane);
+    };
+    planes();
+    const auto piece = [&](int i) {                                   // i < PA: of A, else of B
+        const bool isa = i < PA;
+        const int j = isa ? i : i - PA;
+        const char* base = isa ? as : bs;
+        if (EPI == EPI_GATE && !isa && (((wave + NW * j) * (1024 / ROW) / GW) & 1)) base += g.up_row * g.b.ld * 2;
+        const char* src = base + (isa ? oa[j] : ob[j]);
+        src = (isa ? ka[j] : kb[j]) < left ? src : reinterpret_cast<const char*>(g_zeros);
+        dma16(src, s_base + (uint32_t)(head * TILE + (isa ? 0 : BM * ROW) + (wave + j * NW) * 1024));
+    };
+    const auto requested = [&]() {                                    // all pieces of the step are out
+        head = head + 1 == NBUF ? 0 : head + 1;
+        left -= KT; as += sa * 2; bs += sb * 2;
+        if (P == 3 && ++kt == steps_k) {
+            kt = 0; ++pair;
+            left = pair < 6 ? (int)(k_hi - k_lo) : 0;
+            planes();
         }
     };
 
@@ -255,78 +260,60 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
         for (int m = 0; m < MR; ++m)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[n][m][r] = 0.0f;
-    // A ring of NBUF buffers.  A step is two blocks of 16 k; while block b is multiplied the fragments of block b + 1 are read, across the
-    // step's border too: half way through step t everybody's pieces of step t + 1 have landed (a counted wait -- a __syncthreads would drain
-    // the queue -- and the barrier) and step t has been read by everybody, so step t + NBUF is requested into its buffer
+    // A ring of NBUF buffers.  While a block of 16 k is multiplied the fragments of the next one are read, across the step's border too: before
+    // the last block of step t everybody's pieces of step t + 1 have landed (a counted wait -- a __syncthreads would drain the queue -- and
+    // the barrier) and step t has been read by everybody, so step t + NBUF is requested into its buffer.  The pieces go out BETWEEN the products
+    // of two blocks: a CU drains about 32 bytes per clock into LDS, and a burst of them would hold up the waves' matrix instructions
     struct Frags { E8 a[MR], b[NR]; };
-    const auto read = [&](Frags& f, int buf, int ks) {
+    constexpr int PIECES = PA + PB, FIRST = PIECES / 2;               // pieces of a step before / after the step's border
+    const auto read = [&](Frags& f, int i, int buf, int ks) {          // fragment i of the MR + NR of a block
         const char* const ta = s_all + buf * TILE;
-        const char* const tb = ta + BM * ROW;
-#pragma unroll
-        for (int j = 0; j < NR; ++j) f.b[j] = frag(tb, BK, ROWB, wn, j, ks);
-#pragma unroll
-        for (int j = 0; j < MR; ++j) f.a[j] = frag(ta, AK, ROWA, wm, j, ks);
+        if (i < NR) f.b[i] = frag(ta + BM * ROW, BK, ROWB, wn, i, ks);
+        else f.a[i - NR] = frag(ta, AK, ROWA, wm, i - NR, ks);
     };
-    const auto multiply = [&](const Frags& f) {
+    // the products of one block; between them, in this order, the reads of the next block (ks of buffer buf) and the pieces p0 .. p1 - 1
+    const auto block = [&](const Frags& f, Frags& next, int buf, int ks, int p0, int p1) {
+        constexpr int N = MR * NR, R = MR + NR;
 #pragma unroll
-        for (int m = 0; m < MR; ++m)
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n) acc[n][m] = mfma(f.b[n], f.a[m], acc[n][m]);
-    };
-    // 0x100: LDS reads, 0x8: matrix instructions -- the reads go out between the first products
-    const auto interleave = [&]() {
-        constexpr int READS = MR * (AK == KC ? 1 : 2) + NR * (BK == KC ? 1 : 2), PER = (READS + MR * NR - 2) / (MR * NR - 1);
+            for (int j = R * i / N; j < R * (i + 1) / N; ++j) read(next, j, buf, ks);
 #pragma unroll
-        for (int i = 0; i < MR * NR - 1; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+            for (int j = p0 + (p1 - p0) * i / N; j < p0 + (p1 - p0) * (i + 1) / N; ++j) piece(j);
+            acc[i % NR][i / NR] = mfma(f.b[i % NR], f.a[i / NR], acc[i % NR][i / NR]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    const auto landed = [&](int younger) {                            // all but the `younger` last requested steps of this wave
-        if (younger >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * (PA + PB)) : "memory");
-        else if (younger == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (PA + PB)) : "memory");
-        else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PA + PB) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    };
-    int pair = 0, kt = 0, head = 0, cur = 0;
-    const auto request = [&]() {
-        issue(pair, kt, head);
-        if (++kt == steps_k) { kt = 0; ++pair; }
-        head = head + 1 == NBUF ? 0 : head + 1;
     };
     Frags f0, f1;
-#pragma unroll
-    for (int i = 0; i < NBUF; ++i)
-        if (i < steps) request();
     if (steps) {
-        landed(min(NBUF, steps) - 1);
+#pragma unroll
+        for (int i = 0; i < NBUF; ++i) {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j)
+                if (i < NBUF - 1 || j < FIRST) piece(j);
+            if (i < NBUF - 1) requested();
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * PIECES + FIRST) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        read(f0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < MR + NR; ++i) read(f0, i, 0, 0);
     }
+    int cur = 0;
     for (int t = 0; t < steps; ++t) {
 #pragma unroll
         for (int ks = 0; ks < KT / 16 - 1; ++ks) {
-            read(ks & 1 ? f0 : f1, cur, ks + 1);
-            multiply(ks & 1 ? f1 : f0);
-            interleave();
+            block(ks & 1 ? f1 : f0, ks & 1 ? f0 : f1, cur, ks + 1, FIRST, ks == 0 ? PIECES : FIRST);      // (the rest of step t + NBUF - 1)
+            if (ks == 0) requested();
         }
         const int nxt = cur + 1 == NBUF ? 0 : cur + 1;
-        if (t + 1 < steps) {
-            landed(min(NBUF - 2, steps - 2 - t));
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (t + NBUF < steps) request();
-            __builtin_amdgcn_sched_barrier(0);
-            read(f0, nxt, 0);
-        }
-        multiply(f1);
-        interleave();
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * PIECES) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        block(f1, f0, nxt, 0, 0, FIRST);                              // (behind the last step: reads of zeros, not used)
         cur = nxt;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // the last pieces, before the buffers are used again
 
     // A lane holds row m = lr of C and columns (reg & 3) + 8 (reg >> 2) + 4 lh of each 32 x 32 block: stored from there an instruction
     // touches 32 rows with 16 bytes each.  Every wave turns its 32-row slices over in LDS instead and works along the rows, 4 columns per lane:
@@ -348,6 +335,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
     const auto slice = [&](int mb, int it, auto all_inside) {
         constexpr bool IN = decltype(all_inside)::value;
         const int r = it * RPI + lane / CPL;
+        if (64 % CPL && lane >= RPI * CPL) return;                    // (192 columns: 48 lanes work)
         const int64_t m = m0 + wm + 32 * mb + r;
         float v[4];
         Pack<float, 4>::load(tile + r * OLD + col, v);
@@ -433,13 +421,14 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
         }
     }
     if constexpr (EPI == EPI_DH) {
-        if (!g.sums) return;
+        static_assert(MR == 2, "a wave's rows are one slice of 64");
+        if (!g.sums || m0 + wm >= g.M) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int off = CPL; off < 64; off <<= 1) { sg[i] += __shfl_xor(sg[i], off, 64); su[i] += __shfl_xor(su[i], off, 64); }
             if (lane < CPL && n + i < g.N) {
-                float* o = g.sums + ((int64_t)tm * WM + wave / WN) * 2 * g.N + n + i;
+                float* o = g.sums + (m0 + wm) / (32 * MR) * 2 * g.N + n + i;
                 o[0] = sg[i];
                 o[g.N] = su[i];
             }
@@ -538,47 +527,82 @@ hipError_t operand(Work& w, const void* src, int64_t halves, int64_t R, int64_t 
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
 hipError_t tiles(Prod g, int splits, hipStream_t s) {
     constexpr int BM = 32 * MR * WM, NT = EPI == EPI_GATE ? 16 * NR * WN : 32 * NR * WN;
-    const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M + BM - 1) / BM, gn = (N + NT - 1) / NT;
-    if (!gm || !gn) return hipSuccess;
+    const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M - g.m_base + BM - 1) / BM, gn = (N + NT - 1) / NT;
+    if (gm <= 0 || !gn) return hipSuccess;
     if (gm * gn > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 63) / 64 * 64 : std::max<int64_t>(g.K, 64);
     k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, KT, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
     return hipGetLastError();
 }
-inline int64_t tile_count(int64_t M, int64_t N, int side) { return ((M + side - 1) / side) * ((N + side - 1) / side); }
+// ---- which tiles, and how many shares of the k loop.  A round is one tile on every CU (two of the 128 x 128 ones); its time is modelled as
+// the k loop at the rate measured on full rounds (1.8 us per 64 k of a 256 x 256 tile; the smaller tiles move more operand bytes per
+// product: 5 % and 20 % on top) plus the epilogue's traffic at 4.5 GB/ms.  Two things decide between the shapes: how full the last round is
+// (16 448 x 1536: 256 x 192 tiles are 2 rounds of 0.75, 256 x 256 ones 2 of 1 for 1.5 rounds of work), and the rows behind the last whole
+// tile (257 tokens per image leave 64 of them): as tiles of 256 they can cost a whole round, as a second launch of 128 x 128 tiles
+// about 6 us and their k loop.
+enum { SHAPE_256 = 0, SHAPE_192 = 1, SHAPE_128 = 2 };
+struct Plan { int shape, splits; int64_t main_rows; };              // rows behind main_rows go to a launch of 128 x 128 tiles
 
-// 256 x 256 tiles (8 waves of 64 x 128) where they fill the chip, else 128 x 128 (4 waves of 64 x 64)
-template <int EPI>
-inline bool big_tiles(const Prod& g, int splits) {
-    const int64_t N = EPI == EPI_GATE ? 2 * g.HP : EPI == EPI_DH ? g.HP : g.N;
-    return tile_count(g.M, N, 256) * splits >= 192;
+inline double round_time(int shape, int64_t M, int64_t N, int64_t K, int splits, double out_bytes) {
+    const int bm = shape == SHAPE_128 ? 128 : 256, bn = shape == SHAPE_128 ? 128 : shape == SHAPE_192 ? 192 : 256, slots = shape == SHAPE_128 ? 512 : 256;
+    const int64_t t = (M + bm - 1) / bm * ((N + bn - 1) / bn) * splits;
+    const double work = shape == SHAPE_256 ? 1.0 : shape == SHAPE_192 ? 0.75 * 1.05 : 0.5 * 1.2;
+    const double steps = (double)((K + 64 * splits - 1) / (64 * splits));
+    return (double)((t + slots - 1) / slots) * (steps * 1.8 * work + 4.0) + (double)M * N * out_bytes / 4.5e6;
 }
-// the 64-row slices whose column sums EPI_DH leaves
-template <int EPI>
-inline int64_t row_slices(const Prod& g) { return big_tiles<EPI>(g, 1) ? (g.M + 255) / 256 * 4 : (g.M + 127) / 128 * 2; }
+// out_bytes: what the epilogue moves per element of C; shares are considered where `most` > 1 (each at least 512 deep)
+inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most) {
+    Plan best{SHAPE_128, 1, M};
+    double least = 1e300;
+    for (int z = 1; z <= most && (z == 1 || K / z >= 512); ++z) {
+        const double join = z > 1 ? 5.0 + (double)M * N * 4 * (z + 1) / 4.5e6 : 0.0;
+        for (int shape = SHAPE_256; shape <= SHAPE_128; ++shape) {
+            if (shape == SHAPE_192 && !may_192) continue;
+            const double all = round_time(shape, M, N, K, z, out_bytes) + join;
+            if (all < least) { least = all; best = {shape, z, M}; }
+            const int64_t whole = M / 256 * 256;
+            if (shape == SHAPE_128 || whole == 0 || whole == M || z > 1) continue;
+            const double two = round_time(shape, whole, N, K, z, out_bytes) + round_time(SHAPE_128, M - whole, N, K, z, out_bytes) + 6.0;
+            if (two < least) { least = two; best = {shape, z, whole}; }
+        }
+    }
+    return best;
+}
 
 template <class T, int AK, int BK, int EPI>
-hipError_t product(const Prod& g, int splits, hipStream_t s) {
-    if (big_tiles<EPI>(g, splits)) return tiles<T, AK, BK, EPI, FFN_BIG, FFN_KT, FFN_NB>(g, splits, s);
-    return tiles<T, AK, BK, EPI, 2, 2, 2, 2, FFN_KT, FFN_NB>(g, splits, s);
+hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
+    if constexpr (EPI == EPI_OUT)
+        if (shape == SHAPE_192) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
+    return shape == SHAPE_256 ? tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s) : tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
 }
-
-// shares of a weight gradient's sum over the rows, when its tiles alone do not fill the chip: each at least 512 deep
-inline int k_splits(int64_t M, int64_t N, int64_t K) {
-    const int64_t t = tile_count(M, N, 128);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(t, 1), K / 512, 64}));
+template <class T, int AK, int BK, int EPI>
+hipError_t product(Prod g, const Plan& p, hipStream_t s) {
+    const int64_t M = g.M;
+    g.M = p.main_rows;
+    FFN_TRY((launch_shape<T, AK, BK, EPI>(p.shape, g, p.splits, s)));
+    g.M = M; g.m_base = p.main_rows;
+    return launch_shape<T, AK, BK, EPI>(SHAPE_128, g, p.splits, s);
+}
+// products over the rows of a batch: no split
+template <class T, int AK, int BK, int EPI>
+hipError_t product(const Prod& g, hipStream_t s) {
+    constexpr double es = sizeof(T);
+    const int64_t planes = Mat<T>::P == 3 ? 6 : 1;
+    if (EPI == EPI_GATE) return product<T, AK, BK, EPI>(g, plan_tiles(g.M, 2 * g.HP, g.K * planes, (es + (g.p ? 8 : 0)) / 2, false, 1), s);
+    if (EPI == EPI_DH) return product<T, AK, BK, EPI>(g, plan_tiles(g.M, g.HP, g.K * planes, 8 + 2 * es, false, 1), s);
+    return product<T, AK, BK, EPI>(g, plan_tiles(g.M, g.N, g.K * planes, es, true, 1), s);
 }
 template <class T>
 hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
-    const int z = k_splits(g.M, g.N, g.K);
+    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 512)));
     g.rows_out = rows_out;
-    if (z > 1) g.part = (float*)w.take((size_t)z * rows_out * g.N * 4);
+    if (p.splits > 1) g.part = (float*)w.take((size_t)p.splits * rows_out * g.N * 4);
     if (w.counting()) return hipSuccess;
-    g.vec_out = g.N % 4 == 0 && (z > 1 || aligned16(g.out));
-    FFN_TRY((product<T, KS, KS, EPI_OUT>(g, z, w.s)));
-    if (z == 1) return hipSuccess;
+    g.vec_out = g.N % 4 == 0 && (p.splits > 1 || aligned16(g.out));
+    FFN_TRY((product<T, KS, KS, EPI_OUT>(g, p, w.s)));
+    if (p.splits == 1) return hipSuccess;
     const int64_t n = rows_out * g.N;
-    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, w.s>>>(g.part, z, n, (T*)g.out);
+    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, w.s>>>(g.part, p.splits, n, (T*)g.out);
     return hipGetLastError();
 }
 template <class T>
@@ -616,11 +640,11 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     Prod g{};
     g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
-    FFN_TRY((product<T, KC, KC, EPI_GATE>(g, 1, w.s)));
+    FFN_TRY((product<T, KC, KC, EPI_GATE>(g, w.s)));
     Prod d{};
     d.a = {h, HP, f.M * HP}; d.b = w3; d.ra = f.M; d.rb = f.O; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
     d.vec_out = f.O % 4 == 0 && aligned16(f.y);
-    return product<T, KC, KC, EPI_OUT>(d, 1, w.s);
+    return product<T, KC, KC, EPI_OUT>(d, w.s);
 }
 
 template <class T>
@@ -636,15 +660,15 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     if (hidden) {
         Operand w3;
         FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
-        const int64_t slices = (f.M + 127) / 128 * 4;                 // at most: row slices of 32 rows and more
+        const int64_t slices = (f.M + 63) / 64;                       // (of 64 rows)
         float* sums = all || f.db12 ? (float*)w.take((size_t)slices * 2 * f.H * 4) : nullptr;
         if (!all) {
             Prod g{};
             g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = GL;
             g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
             g.sums = sums;
-            FFN_TRY((product<T, KC, KS, EPI_DH>(g, 1, w.s)));
-            if (f.db12) FFN_TRY(join_columns<T>(sums, row_slices<EPI_DH>(g), 2 * (int64_t)f.H, f.db12, w.s));
+            FFN_TRY((product<T, KC, KS, EPI_DH>(g, w.s)));
+            if (f.db12) FFN_TRY(join_columns<T>(sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
         }
     }
     if (all || f.dx) {
@@ -653,7 +677,7 @@ hipError_t backward(const FfnArgs& f, Work& w) {
         if (!all) {
             Prod g{};
             g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
-            FFN_TRY((product<T, KC, KS, EPI_OUT>(g, 1, w.s)));
+            FFN_TRY((product<T, KC, KS, EPI_OUT>(g, w.s)));
         }
     }
     if (all || f.dw12) {
