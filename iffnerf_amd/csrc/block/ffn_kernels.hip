@@ -135,11 +135,14 @@ struct Prod {
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
 
-// 16 bytes per lane from `src` to LDS, lane-linear from byte `lds` on.  As assembly: behind the builtin the compiler drains the memory queue
-// before every transposed LDS read (it takes the two for aliases), which serialised the products with a k-strided operand (dW12 at
-// 16448 x 1536 x 4096: 745 against 497 us).  Nothing is returned to a register; the waits are the kernel's own counted ones.
+// 16 bytes per lane from `src` to LDS, lane-linear from byte `lds` on.  TR: as assembly -- behind the builtin the compiler drains the memory
+// queue before every transposed LDS read (it takes the two for aliases), which serialised the products with a k-strided operand (dW12 at
+// 16448 x 1536 x 4096: 745 against 369 us); beside plain reads the builtin is the faster form (F2: 219 against 245 us).  Nothing is
+// returned to a register; the waits are the kernel's own counted ones.  (Nothing else in these kernels uses m0.)
+template <bool TR>
 __device__ __forceinline__ void dma16(const char* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");      // (nothing else in these kernels uses m0)
+    if constexpr (TR) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
+    else __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(uintptr_t)lds, 16, 0, 0);
 }
 
 // Workgroups are dealt round-robin over the 8 XCDs, each with its own L2.  The ones that share an XCD (ids equal mod 8) take a contiguous
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
         if (EPI == EPI_GATE && !isa && (((wave + NW * j) * (1024 / ROW) / GW) & 1)) base += g.up_row * g.b.ld * 2;
         const char* src = base + (isa ? oa[j] : ob[j]);
         src = (isa ? ka[j] : kb[j]) < left ? src : reinterpret_cast<const char*>(g_zeros);
-        dma16(src, s_base + (uint32_t)(head * TILE + (isa ? 0 : BM * ROW) + (wave + j * NW) * 1024));
+        dma16<AK == KS || BK == KS>(src, s_base + (uint32_t)(head * TILE + (isa ? 0 : BM * ROW) + (wave + j * NW) * 1024));
     };
     const auto requested = [&]() {                                    // all pieces of the step are out
         head = head + 1 == NBUF ? 0 : head + 1;
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
             }
             const bool vec = IN || (g.vec_out && n < g.N);
             if (g.part) {
-                float* o = g.part + (blockIdx.y * g.rows_out + row) * g.N + n;
+                float* o = g.part + (blockIdx.y * g.rows_out + row - g.m_base) * g.N + n;
                 if (vec) Pack<float, 4>::store(o, v);
                 else
 #pragma unroll
@@ -436,13 +439,14 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
     }
 }
 
-// out[i] = sum_z part[z][i] in increasing z
+// out[i] = sum_z part[z][i] in increasing z (+ bias of the column, N columns)
 template <class T>
-__global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part, int Z, int64_t n, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part, int Z, int64_t n, int64_t N, const T* __restrict__ bias,
+                                                  T* __restrict__ out) {
     for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float v = part[i];
         for (int z = 1; z < Z; ++z) v += part[z * n + i];
-        out[i] = (T)v;
+        out[i] = (T)(bias ? v + (float)bias[i % N] : v);
     }
 }
 
@@ -541,7 +545,7 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
 // tile (257 tokens per image leave 64 of them): as tiles of 256 they can cost a whole round, as a second launch of 128 x 128 tiles
 // about 6 us and their k loop.
 enum { SHAPE_256 = 0, SHAPE_192 = 1, SHAPE_128 = 2 };
-struct Plan { int shape, splits; int64_t main_rows; };              // rows behind main_rows go to a launch of 128 x 128 tiles
+struct Plan { int shape, splits; int64_t main_rows; int rest_splits; };      // rows behind main_rows go to a launch of 128 x 128 tiles
 
 inline double round_time(int shape, int64_t M, int64_t N, int64_t K, int splits, double out_bytes) {
     const int bm = shape == SHAPE_128 ? 128 : 256, bn = shape == SHAPE_128 ? 128 : shape == SHAPE_192 ? 192 : 256, slots = shape == SHAPE_128 ? 512 : 256;
@@ -550,20 +554,27 @@ inline double round_time(int shape, int64_t M, int64_t N, int64_t K, int splits,
     const double steps = (double)((K + 64 * splits - 1) / (64 * splits));
     return (double)((t + slots - 1) / slots) * (steps * 1.8 * work + 4.0) + (double)M * N * out_bytes / 4.5e6;
 }
-// out_bytes: what the epilogue moves per element of C; shares are considered where `most` > 1 (each at least 512 deep)
-inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most) {
-    Plan best{SHAPE_128, 1, M};
+// out_bytes: what the epilogue moves per element of C; most: shares of the k loop that may be taken (each at least 512 deep); most_rest: those of
+// the remainder's launch (at least 256 deep)
+inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most, int most_rest) {
+    Plan best{SHAPE_128, 1, M, 1};
     double least = 1e300;
+    const int64_t whole = M / 256 * 256;
+    double rest = 1e300;                                          // the remainder's launch
+    int rest_splits = 1;
+    for (int z = 1; whole && whole < M && z <= most_rest && (z == 1 || K / z >= 256); ++z) {
+        const double t = 6.0 + round_time(SHAPE_128, M - whole, N, K, z, out_bytes) + (z > 1 ? 5.0 + (double)(M - whole) * N * 4 * (z + 1) / 4.5e6 : 0.0);
+        if (t < rest) { rest = t; rest_splits = z; }
+    }
     for (int z = 1; z <= most && (z == 1 || K / z >= 512); ++z) {
         const double join = z > 1 ? 5.0 + (double)M * N * 4 * (z + 1) / 4.5e6 : 0.0;
         for (int shape = SHAPE_256; shape <= SHAPE_128; ++shape) {
             if (shape == SHAPE_192 && !may_192) continue;
             const double all = round_time(shape, M, N, K, z, out_bytes) + join;
-            if (all < least) { least = all; best = {shape, z, M}; }
-            const int64_t whole = M / 256 * 256;
-            if (shape == SHAPE_128 || whole == 0 || whole == M || z > 1) continue;
-            const double two = round_time(shape, whole, N, K, z, out_bytes) + round_time(SHAPE_128, M - whole, N, K, z, out_bytes) + 6.0;
-            if (two < least) { least = two; best = {shape, z, whole}; }
+            if (all < least) { least = all; best = {shape, z, M, 1}; }
+            if (shape == SHAPE_128 || z > 1 || whole == 0 || whole == M) continue;
+            const double two = round_time(shape, whole, N, K, z, out_bytes) + rest;
+            if (two < least) { least = two; best = {shape, z, whole, rest_splits}; }
         }
     }
     return best;
@@ -575,35 +586,43 @@ hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
         if (shape == SHAPE_192) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
     return shape == SHAPE_256 ? tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s) : tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
 }
-template <class T, int AK, int BK, int EPI>
-hipError_t product(Prod g, const Plan& p, hipStream_t s) {
-    const int64_t M = g.M;
-    g.M = p.main_rows;
-    FFN_TRY((launch_shape<T, AK, BK, EPI>(p.shape, g, p.splits, s)));
-    g.M = M; g.m_base = p.main_rows;
-    return launch_shape<T, AK, BK, EPI>(SHAPE_128, g, p.splits, s);
+template <class T>
+hipError_t join_shares(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out, hipStream_t s) {
+    const int64_t n = rows * N;
+    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, s>>>(part, z, n, N, (const T*)bias, (T*)out);
+    return hipGetLastError();
 }
-// products over the rows of a batch: no split
+// a product over the rows of a batch; the k loop of its main launch is not split
 template <class T, int AK, int BK, int EPI>
-hipError_t product(const Prod& g, hipStream_t s) {
+hipError_t product(Work& w, Prod g) {
     constexpr double es = sizeof(T);
-    const int64_t planes = Mat<T>::P == 3 ? 6 : 1;
-    if (EPI == EPI_GATE) return product<T, AK, BK, EPI>(g, plan_tiles(g.M, 2 * g.HP, g.K * planes, (es + (g.p ? 8 : 0)) / 2, false, 1), s);
-    if (EPI == EPI_DH) return product<T, AK, BK, EPI>(g, plan_tiles(g.M, g.HP, g.K * planes, 8 + 2 * es, false, 1), s);
-    return product<T, AK, BK, EPI>(g, plan_tiles(g.M, g.N, g.K * planes, es, true, 1), s);
+    const int64_t K = g.K * (Mat<T>::P == 3 ? 6 : 1), M = g.M;
+    const Plan p = EPI == EPI_GATE ? plan_tiles(M, 2 * g.HP, K, (es + (g.p ? 8 : 0)) / 2, false, 1, 1)
+                 : EPI == EPI_DH   ? plan_tiles(M, g.HP, K, 8 + 2 * es, false, 1, 1)
+                                   : plan_tiles(M, g.N, K, es, true, 1, 16);
+    const int64_t rest = M - p.main_rows;
+    float* part = p.rest_splits > 1 ? (float*)w.take((size_t)p.rest_splits * rest * g.N * 4) : nullptr;
+    if (w.counting()) return hipSuccess;
+    g.M = p.main_rows;
+    FFN_TRY((launch_shape<T, AK, BK, EPI>(p.shape, g, 1, w.s)));
+    if (!rest) return hipSuccess;
+    g.M = M; g.m_base = p.main_rows;
+    if (!part) return launch_shape<T, AK, BK, EPI>(SHAPE_128, g, 1, w.s);
+    g.part = part; g.rows_out = rest;                                // shares of the rows behind m_base
+    void* out = (T*)g.out + p.main_rows * g.N;
+    g.vec_out = g.N % 4 == 0;
+    FFN_TRY((launch_shape<T, AK, BK, EPI>(SHAPE_128, g, p.rest_splits, w.s)));
+    return join_shares<T>(part, p.rest_splits, rest, g.N, g.bias, out, w.s);
 }
 template <class T>
 hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
-    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 512)));
+    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 512)), 0);
     g.rows_out = rows_out;
     if (p.splits > 1) g.part = (float*)w.take((size_t)p.splits * rows_out * g.N * 4);
     if (w.counting()) return hipSuccess;
     g.vec_out = g.N % 4 == 0 && (p.splits > 1 || aligned16(g.out));
-    FFN_TRY((product<T, KS, KS, EPI_OUT>(g, p, w.s)));
-    if (p.splits == 1) return hipSuccess;
-    const int64_t n = rows_out * g.N;
-    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, w.s>>>(g.part, p.splits, n, (T*)g.out);
-    return hipGetLastError();
+    FFN_TRY((launch_shape<T, KS, KS, EPI_OUT>(p.shape, g, p.splits, w.s)));
+    return p.splits > 1 ? join_shares<T>(g.part, p.splits, rows_out, g.N, nullptr, g.out, w.s) : hipSuccess;
 }
 template <class T>
 hipError_t join_columns(const float* part, int64_t G, int64_t N, void* out, hipStream_t s) {
@@ -636,15 +655,14 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
     char* h = (char*)f.kept;
     if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
-    if (w.counting()) return hipSuccess;
     Prod g{};
     g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
-    FFN_TRY((product<T, KC, KC, EPI_GATE>(g, w.s)));
+    FFN_TRY((product<T, KC, KC, EPI_GATE>(w, g)));
     Prod d{};
     d.a = {h, HP, f.M * HP}; d.b = w3; d.ra = f.M; d.rb = f.O; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
     d.vec_out = f.O % 4 == 0 && aligned16(f.y);
-    return product<T, KC, KC, EPI_OUT>(d, w.s);
+    return product<T, KC, KC, EPI_OUT>(w, d);
 }
 
 template <class T>
@@ -662,22 +680,22 @@ hipError_t backward(const FfnArgs& f, Work& w) {
         FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
         const int64_t slices = (f.M + 63) / 64;                       // (of 64 rows)
         float* sums = all || f.db12 ? (float*)w.take((size_t)slices * 2 * f.H * 4) : nullptr;
-        if (!all) {
+        {
             Prod g{};
             g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = GL;
             g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
             g.sums = sums;
-            FFN_TRY((product<T, KC, KS, EPI_DH>(g, w.s)));
-            if (f.db12) FFN_TRY(join_columns<T>(sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
+            FFN_TRY((product<T, KC, KS, EPI_DH>(w, g)));
+            if (!all && f.db12) FFN_TRY(join_columns<T>(sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
         }
     }
     if (all || f.dx) {
         Operand w12;
         FFN_TRY(operand<T>(w, f.w12, 2, f.H, f.D, w12));
-        if (!all) {
+        {
             Prod g{};
             g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
-            FFN_TRY((product<T, KC, KS, EPI_OUT>(g, w.s)));
+            FFN_TRY((product<T, KC, KS, EPI_OUT>(w, g)));
         }
     }
     if (all || f.dw12) {
