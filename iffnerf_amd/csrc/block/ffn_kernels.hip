@@ -83,25 +83,32 @@ __device__ __forceinline__ void store4(T* o, const float v[4]) {
 
 __host__ __device__ constexpr int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind column C and behind row R of a half; 8 columns per thread
+// Up to four matrices in one launch, job j from workgroup first[j] on: src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind
+// column C and behind row R of a half; 8 columns per thread
+struct PackJob { const void* src; void* dst; int64_t R, RP, C, CP, rows_out; int vec; };
+struct PackJobs { PackJob job[4]; unsigned first[5]; int n; };
 template <class T>
-__global__ void __launch_bounds__(256) k_ffn_pack(const T* __restrict__ src, int64_t R, int64_t RP, int64_t C, int64_t CP, int64_t rows_out, bool vec,
-                                                  typename Mat<T>::e* __restrict__ dst) {
+__global__ void __launch_bounds__(256) k_ffn_pack(PackJobs jobs) {
     typedef typename Mat<T>::e E;
     typedef typename Vec8<E>::t E8;
     constexpr int P = Mat<T>::P;
-    const int64_t cols8 = CP / 8, n = rows_out * cols8;
-    for (int64_t t = blockIdx.x * (int64_t)256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-        const int64_t row = t / cols8, c0 = (t - row * cols8) * 8;
-        const int64_t half = row / RP, r = row - half * RP;
+    int k = 0;
+    while (k + 1 < jobs.n && blockIdx.x >= jobs.first[k + 1]) ++k;
+    const PackJob j = jobs.job[k];
+    const unsigned wgs = jobs.first[k + 1] - jobs.first[k];
+    const int64_t cols8 = j.CP / 8, n = j.rows_out * cols8;
+    E* const dst = reinterpret_cast<E*>(j.dst);
+    for (int64_t t = (blockIdx.x - jobs.first[k]) * (int64_t)256 + threadIdx.x; t < n; t += (int64_t)wgs * 256) {
+        const int64_t row = n < (1ll << 31) ? (int64_t)((uint32_t)t / (uint32_t)cols8) : t / cols8, c0 = (t - row * cols8) * 8;
+        const int64_t half = row >= j.RP, r = row - half * j.RP;
         float v[8];
-        const T* s = src + (half * R + r) * C + c0;
-        if (vec && r < R) {
+        const T* s = reinterpret_cast<const T*>(j.src) + (half * j.R + r) * j.C + c0;
+        if (j.vec && r < j.R) {
 #pragma unroll
             for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) Pack<T, 16 / sizeof(T)>::load(s + i, v + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = r < R && c0 + i < C ? (float)s[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = r < j.R && c0 + i < j.C ? (float)s[i] : 0.0f;
         }
         E8 o[P];
 #pragma unroll
@@ -112,7 +119,7 @@ __global__ void __launch_bounds__(256) k_ffn_pack(const T* __restrict__ src, int
             for (int p = 0; p < P; ++p) o[p][i] = e[p];
         }
 #pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<E8*>(dst + p * rows_out * CP + row * CP + c0) = o[p];
+        for (int p = 0; p < P; ++p) *reinterpret_cast<E8*>(dst + p * j.rows_out * j.CP + row * j.CP + c0) = o[p];
     }
 }
 
@@ -129,7 +136,7 @@ struct Prod {
     void* out; const void* bias; float* part; int64_t half_pad, half, rows_out; bool vec_out;
     // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld ldo; factors p, q [M][HP = pad8(H)] or null; bias b12
     // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
-    // and with `sums`: [M / 64][2H] column sums of dg and du (fp32, before they are rounded) over 64 rows each
+    // and with `sums`: [M / 32 MR][2H] column sums of dg and du (fp32, before they are rounded) over a wave's rows
     int64_t up_row, HP, ldo; float* p; float* q; int act; float* sums;
 };
 
@@ -158,11 +165,11 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
 
 // Tiles of 32 MR WM x 32 NR WN, 32 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
 // 1 KB per instruction, lane-linear in LDS) into a ring of NBUF buffers.  A KC tile is rows of 32 k
-// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k (64 or 128 chunks of m), chunk c in slot
-// c ^ 4 (k & 3), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
+// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 columns,
+// two rows per 256 bytes: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
 // keep every LDS read free of bank conflicts.
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
+__global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
     typedef typename Mat<T>::e E;
     typedef typename Vec8<E>::t E8;
     constexpr int P = Mat<T>::P, NW = WM * WN, BM = 32 * MR * WM, BN = 32 * NR * WN;
@@ -183,6 +190,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
     const E* const B = reinterpret_cast<const E*>(g.b.p);
 
     const auto swizzle = [](int r) { return KT == 64 ? (r >> 1) & 7 : (r >> 2) & 3; };
+    const auto turn = [](int r, int width) { return width == 64 ? (r & 2) << 1 : (r & 3) << 2; };
 
     // the lane's source of each piece, in bytes from the tile's corner at the step's k (ld < 2^22: 256 rows stay below 2^31), and its first k
     uint32_t oa[PA], ob[PB];
@@ -190,14 +198,14 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
 #pragma unroll
     for (int i = 0; i < PA; ++i) {
         const int at = (wave + NW * i) * 1024 + lane * 16;
-        const int r = at / (AK == KC ? ROW : BM * 2), c = ((at % (AK == KC ? ROW : BM * 2)) >> 4) ^ (AK == KC ? swizzle(r) : (r & 3) << 2);
+        const int r = at / (AK == KC ? ROW : BM * 2), c = ((at % (AK == KC ? ROW : BM * 2)) >> 4) ^ (AK == KC ? swizzle(r) : turn(r, BM));
         if (AK == KC) { oa[i] = (uint32_t)((min(m0 + r, g.ra - 1) - m0) * g.a.ld + c * 8) * 2; ka[i] = c * 8; }
         else { oa[i] = (uint32_t)(r * g.a.ld + min(m0 + c * 8, g.a.ld - 8) - m0) * 2; ka[i] = r; }
     }
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
         const int at = (wave + NW * i) * 1024 + lane * 16;
-        const int r = at / (BK == KC ? ROW : BN * 2), c = ((at % (BK == KC ? ROW : BN * 2)) >> 4) ^ (BK == KC ? swizzle(r) : (r & 3) << 2);
+        const int r = at / (BK == KC ? ROW : BN * 2), c = ((at % (BK == KC ? ROW : BN * 2)) >> 4) ^ (BK == KC ? swizzle(r) : turn(r, BN));
         if (BK == KC) {
             // a gate tile's rows, per wave: GW gate rows, then the up rows of the same hidden units
             const int64_t row = EPI == EPI_GATE ? min(n0 + r / (2 * GW) * GW + r % GW, g.N - 1) : min(n0 + r, g.rb - 1);
@@ -243,13 +251,13 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
 
     // where this lane's fragments are in a tile: KC one 16-byte read per 16 k, KS two transposed 8-byte reads
     constexpr int ROWA = AK == KC ? ROW : BM * 2, ROWB = BK == KC ? ROW : BN * 2;
-    const int sw = swizzle(lr), trow = 8 * lh + ((lane & 15) >> 2), tx = ((lane >> 2) & 3) << 2;
+    const int sw = swizzle(lr), trow = 8 * lh + ((lane & 15) >> 2);
     const int tcol = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
     auto frag = [&](const char* tile, int kind, int rowbytes, int base, int j, int ks) -> E8 {
         if (kind == KC) return *reinterpret_cast<const E8*>(tile + (base + 32 * j + lr) * ROW + (((2 * ks + lh) ^ sw) << 4));
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const char* at = tile + (16 * ks + trow) * rowbytes + (((base / 8 + 4 * j) ^ tx) << 4) + tcol;
+        const char* at = tile + (16 * ks + trow) * rowbytes + (((base / 8 + 4 * j) ^ turn(trow, rowbytes / 2)) << 4) + tcol;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 4 * rowbytes));
         const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -424,7 +432,6 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
         }
     }
     if constexpr (EPI == EPI_DH) {
-        static_assert(MR == 2, "a wave's rows are one slice of 64");
         if (!g.sums || m0 + wm >= g.M) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -437,6 +444,67 @@ __global__ void __launch_bounds__(64 * WM * WN, MR * NR >= 16 ? 1 : 2) k_ffn_pro
             }
         }
     }
+}
+
+// ------------------------------------------------------------------------------------------------ a few tokens
+// At most 8 rows and no gradients (serving token by token): the weights are read once and that is all the time there is, so the products are
+// vector dot products -- a wave per RW rows of the weight matrix, its lanes over k, 16 bytes per load, fp32 sums joined across the lanes --
+// and not tiles of which 8 of 128 rows would be used.  GATE: RW / 2 hidden units, their gate and their up row; else RW outputs.
+template <class T, int V, int MM, int RW, bool GATE>
+__global__ void __launch_bounds__(256) k_ffn_few(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, int64_t N, const T* __restrict__ bias,
+                                                 int act, T* __restrict__ out) {
+    constexpr int U = GATE ? RW / 2 : RW;                            // columns of the output per wave
+    const int lane = threadIdx.x & 63;
+    const int64_t n0 = (blockIdx.x * (int64_t)4 + (threadIdx.x >> 6)) * U;
+    if (n0 >= N) return;
+    const T* row[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+        const int64_t n = min(n0 + r % U, N - 1);
+        row[r] = w + (GATE && r >= U ? N + n : n) * K;
+    }
+    float acc[RW][MM];
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+#pragma unroll
+        for (int m = 0; m < MM; ++m) acc[r][m] = 0.0f;
+#pragma unroll 2
+    for (int64_t k = lane * V; k < K; k += 64 * V) {
+        float a[RW][V];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) Pack<T, V>::load(row[r] + k, a[r]);
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            float b[V];
+            Pack<T, V>::load(x + min(m, M - 1) * K + k, b);
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[r][m] = fmaf(a[r][i], b[i], acc[r][m]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+#pragma unroll
+        for (int m = 0; m < MM; ++m)
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) acc[r][m] += __shfl_xor(acc[r][m], off, 64);
+    // lane u MM + m writes output column n0 + u of row m
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            const int64_t n = n0 + u;
+            if (lane != u * MM + m || m >= M || n >= N) continue;
+            float v = acc[u][m] + (bias ? (float)bias[n] : 0.0f);
+            if constexpr (GATE) {
+                const float up = acc[U + u][m] + (bias ? (float)bias[N + n] : 0.0f);
+                float f, df;
+                activation<Mat<T>::P == 3>(act, v, f, df);
+                v = f * up;
+            }
+            out[m * N + n] = (T)v;
+        }
 }
 
 // out[i] = sum_z part[z][i] in increasing z (+ bias of the column, N columns)
@@ -509,24 +577,31 @@ struct Work {
 
 template <class T> inline size_t planes_bytes(int64_t rows, int64_t ld) { return (size_t)rows * ld * Mat<T>::P * 2; }
 
-// src [halves x R][C] as an operand: itself, or packed
+// the matrices a call multiplies, each as itself or packed by one launch for all of them
 template <class T>
-hipError_t operand(Work& w, const void* src, int64_t halves, int64_t R, int64_t C, Operand& o) {
-    const int64_t RP = halves > 1 ? pad8(R) : R, CP = pad8(C), rows = halves * RP;
-    o.ld = CP; o.plane = rows * CP; o.p = src;
-    if (Mat<T>::P == 1 && CP == C && RP == R && (w.counting() || aligned16(src))) {
-        // (counting: a start that is not 16-byte aligned is copied too, and the size must not depend on it)
-        if (w.counting()) w.take(planes_bytes<T>(rows, CP));
-        return hipSuccess;
+struct Packer {
+    Work& w;
+    PackJobs jobs{};
+    explicit Packer(Work& work) : w(work) {}
+    // src [halves x R][C]; where the size is counted the copy is too (whether a start is 16-byte aligned must not change it)
+    Operand add(const void* src, int64_t halves, int64_t R, int64_t C) {
+        const int64_t RP = halves > 1 ? pad8(R) : R, CP = pad8(C), rows = halves * RP;
+        if (Mat<T>::P == 1 && CP == C && RP == R && !w.counting() && aligned16(src)) return {src, CP, rows * CP};
+        void* dst = w.take(planes_bytes<T>(rows, CP));
+        if (!w.counting() && rows) {
+            const int64_t n = rows * CP / 8;
+            jobs.job[jobs.n] = {src, dst, R, RP, C, CP, rows, aligned16(src) && CP == C};
+            jobs.first[jobs.n + 1] = jobs.first[jobs.n] + (unsigned)std::min<int64_t>((n + 255) / 256, 4096);
+            ++jobs.n;
+        }
+        return {dst, CP, rows * CP};
     }
-    void* dst = w.take(planes_bytes<T>(rows, CP));
-    o.p = dst;
-    if (w.counting() || rows == 0) return hipSuccess;
-    const int64_t n = rows * CP / 8;
-    k_ffn_pack<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192), 256, 0, w.s>>>((const T*)src, R, RP, C, CP, rows, aligned16(src) && CP == C,
-                                                                                       (typename Mat<T>::e*)dst);
-    return hipGetLastError();
-}
+    hipError_t go() {
+        if (!jobs.n) return hipSuccess;
+        k_ffn_pack<T><<<jobs.first[jobs.n], 256, 0, w.s>>>(jobs);
+        return hipGetLastError();
+    }
+};
 
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
 hipError_t tiles(Prod g, int splits, hipStream_t s) {
@@ -544,47 +619,55 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
 // (16 448 x 1536: 256 x 192 tiles are 2 rounds of 0.75, 256 x 256 ones 2 of 1 for 1.5 rounds of work), and the rows behind the last whole
 // tile (257 tokens per image leave 64 of them): as tiles of 256 they can cost a whole round, as a second launch of 128 x 128 tiles
 // about 6 us and their k loop.
-enum { SHAPE_256 = 0, SHAPE_192 = 1, SHAPE_128 = 2 };
-struct Plan { int shape, splits; int64_t main_rows; int rest_splits; };      // rows behind main_rows go to a launch of 128 x 128 tiles
+// A product with few tiles is bound by the latency of its steps instead: 0.85 us per 64 k of a 128 x 128 tile alone on its CU with two buffers,
+// less with four (then the tile has the CU to itself), and 64 x 64 tiles bring four times the workgroups.
+enum { SHAPE_256 = 0, SHAPE_192, SHAPE_128, SHAPE_128_DEEP, SHAPE_64, SHAPES };
+constexpr struct Shape { int bm, bn, slots; double step; } kShape[SHAPES] = {          // step: us per 64 k of a round
+    {256, 256, 256, 1.8}, {256, 192, 256, 1.42}, {128, 128, 512, 1.08}, {128, 128, 256, 0.60}, {64, 64, 512, 0.45}};
+struct Plan { int shape, splits; int64_t main_rows; int rest_shape, rest_splits; };      // the rows behind main_rows go to a launch of their own
 
 inline double round_time(int shape, int64_t M, int64_t N, int64_t K, int splits, double out_bytes) {
-    const int bm = shape == SHAPE_128 ? 128 : 256, bn = shape == SHAPE_128 ? 128 : shape == SHAPE_192 ? 192 : 256, slots = shape == SHAPE_128 ? 512 : 256;
-    const int64_t t = (M + bm - 1) / bm * ((N + bn - 1) / bn) * splits;
-    const double work = shape == SHAPE_256 ? 1.0 : shape == SHAPE_192 ? 0.75 * 1.05 : 0.5 * 1.2;
+    const Shape& s = kShape[shape];
+    const int64_t t = (M + s.bm - 1) / s.bm * ((N + s.bn - 1) / s.bn) * splits;
     const double steps = (double)((K + 64 * splits - 1) / (64 * splits));
-    return (double)((t + slots - 1) / slots) * (steps * 1.8 * work + 4.0) + (double)M * N * out_bytes / 4.5e6;
+    return (double)((t + s.slots - 1) / s.slots) * (steps * s.step + 3.0) + (double)M * N * out_bytes / 4.5e6;
 }
-// out_bytes: what the epilogue moves per element of C; most: shares of the k loop that may be taken (each at least 512 deep); most_rest: those of
-// the remainder's launch (at least 256 deep)
-inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most, int most_rest) {
-    Plan best{SHAPE_128, 1, M, 1};
-    double least = 1e300;
-    const int64_t whole = M / 256 * 256;
-    double rest = 1e300;                                          // the remainder's launch
-    int rest_splits = 1;
-    for (int z = 1; whole && whole < M && z <= most_rest && (z == 1 || K / z >= 256); ++z) {
-        const double t = 6.0 + round_time(SHAPE_128, M - whole, N, K, z, out_bytes) + (z > 1 ? 5.0 + (double)(M - whole) * N * 4 * (z + 1) / 4.5e6 : 0.0);
-        if (t < rest) { rest = t; rest_splits = z; }
-    }
-    for (int z = 1; z <= most && (z == 1 || K / z >= 512); ++z) {
-        const double join = z > 1 ? 5.0 + (double)M * N * 4 * (z + 1) / 4.5e6 : 0.0;
-        for (int shape = SHAPE_256; shape <= SHAPE_128; ++shape) {
+inline double share_time(int64_t M, int64_t N, int splits) { return splits > 1 ? 5.0 + (double)M * N * 4 * (splits + 1) / 4.5e6 : 0.0; }
+// out_bytes: what the epilogue moves per element of C; most: shares of the k loop that may be taken, each at least 256 deep
+inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most, bool may_rest = true) {
+    Plan best{SHAPE_128, 1, M, SHAPE_128, 1};
+    double least = 1e300, rest = 1e300;
+    const int64_t whole = may_rest ? M / 256 * 256 : 0;
+    int rest_shape = SHAPE_128, rest_splits = 1;
+    for (int z = 1; z <= most && (z == 1 || K / z >= 256); ++z)
+        for (int shape = SHAPE_256; shape < SHAPES; ++shape) {
             if (shape == SHAPE_192 && !may_192) continue;
-            const double all = round_time(shape, M, N, K, z, out_bytes) + join;
-            if (all < least) { least = all; best = {shape, z, M, 1}; }
-            if (shape == SHAPE_128 || z > 1 || whole == 0 || whole == M) continue;
-            const double two = round_time(shape, whole, N, K, z, out_bytes) + rest;
-            if (two < least) { least = two; best = {shape, z, whole, rest_splits}; }
+            const double all = round_time(shape, M, N, K, z, out_bytes) + share_time(M, N, z);
+            if (all < least) { least = all; best = {shape, z, M, SHAPE_128, 1}; }
+            if (!whole || whole == M || shape < SHAPE_128 || z > 16) continue;
+            const double t = 6.0 + round_time(shape, M - whole, N, K, z, out_bytes) + share_time(M - whole, N, z);
+            if (t < rest) { rest = t; rest_shape = shape; rest_splits = z; }
         }
-    }
+    if (whole && whole < M)
+        for (int shape = SHAPE_256; shape <= SHAPE_192; ++shape) {
+            if (shape == SHAPE_192 && !may_192) continue;
+            const double two = round_time(shape, whole, N, K, 1, out_bytes) + rest;
+            if (two < least) { least = two; best = {shape, 1, whole, rest_shape, rest_splits}; }
+        }
     return best;
 }
 
 template <class T, int AK, int BK, int EPI>
 hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
-    if constexpr (EPI == EPI_OUT)
-        if (shape == SHAPE_192) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
-    return shape == SHAPE_256 ? tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s) : tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
+    switch (shape) {
+    case SHAPE_256: return tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s);
+    case SHAPE_192:
+        if constexpr (EPI == EPI_OUT) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
+        return hipErrorInvalidConfiguration;
+    case SHAPE_128: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
+    case SHAPE_128_DEEP: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 4>(g, splits, s);
+    default: return tiles<T, AK, BK, EPI, 2, 2, 1, 1, 64, 4>(g, splits, s);
+    }
 }
 template <class T>
 hipError_t join_shares(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out, hipStream_t s) {
@@ -592,31 +675,40 @@ hipError_t join_shares(const float* part, int z, int64_t rows, int64_t N, const 
     k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, s>>>(part, z, n, N, (const T*)bias, (T*)out);
     return hipGetLastError();
 }
-// a product over the rows of a batch; the k loop of its main launch is not split
+// rows `from` .. M - 1 of a product, over `splits` shares of k
+template <class T, int AK, int BK, int EPI>
+hipError_t rows_of(Work& w, Prod g, int64_t from, int shape, int splits) {
+    float* part = splits > 1 ? (float*)w.take((size_t)splits * (g.M - from) * g.N * 4) : nullptr;
+    if (w.counting() || from == g.M) return hipSuccess;
+    g.m_base = from;
+    if (!part) return launch_shape<T, AK, BK, EPI>(shape, g, 1, w.s);
+    g.part = part; g.rows_out = g.M - from; g.vec_out = g.N % 4 == 0;
+    FFN_TRY((launch_shape<T, AK, BK, EPI>(shape, g, splits, w.s)));
+    return join_shares<T>(part, splits, g.M - from, g.N, g.bias, (T*)g.out + from * g.N, w.s);
+}
+template <class T, int EPI>
+Plan product_plan(const Prod& g) {
+    constexpr double es = sizeof(T);
+    const int64_t K = g.K * (Mat<T>::P == 3 ? 6 : 1);
+    if (EPI == EPI_GATE) return plan_tiles(g.M, 2 * g.HP, K, (es + (g.p ? 8 : 0)) / 2, false, 1);
+    if (EPI == EPI_OUT) return plan_tiles(g.M, g.N, K, es, true, (int)std::max<int64_t>(1, std::min<int64_t>(16, g.K / 64)));
+    Plan p = plan_tiles(g.M, g.HP, K, 8 + 2 * es, false, 1);
+    if (p.rest_shape == SHAPE_64) p.rest_shape = SHAPE_128_DEEP;     // (one height of the waves' rows, that of the sums, per product)
+    return p;
+}
+// a product over the rows of a batch
 template <class T, int AK, int BK, int EPI>
 hipError_t product(Work& w, Prod g) {
-    constexpr double es = sizeof(T);
-    const int64_t K = g.K * (Mat<T>::P == 3 ? 6 : 1), M = g.M;
-    const Plan p = EPI == EPI_GATE ? plan_tiles(M, 2 * g.HP, K, (es + (g.p ? 8 : 0)) / 2, false, 1, 1)
-                 : EPI == EPI_DH   ? plan_tiles(M, g.HP, K, 8 + 2 * es, false, 1, 1)
-                                   : plan_tiles(M, g.N, K, es, true, 1, 16);
-    const int64_t rest = M - p.main_rows;
-    float* part = p.rest_splits > 1 ? (float*)w.take((size_t)p.rest_splits * rest * g.N * 4) : nullptr;
-    if (w.counting()) return hipSuccess;
+    const Plan p = product_plan<T, EPI>(g);
+    const int64_t M = g.M;
     g.M = p.main_rows;
-    FFN_TRY((launch_shape<T, AK, BK, EPI>(p.shape, g, 1, w.s)));
-    if (!rest) return hipSuccess;
-    g.M = M; g.m_base = p.main_rows;
-    if (!part) return launch_shape<T, AK, BK, EPI>(SHAPE_128, g, 1, w.s);
-    g.part = part; g.rows_out = rest;                                // shares of the rows behind m_base
-    void* out = (T*)g.out + p.main_rows * g.N;
-    g.vec_out = g.N % 4 == 0;
-    FFN_TRY((launch_shape<T, AK, BK, EPI>(SHAPE_128, g, p.rest_splits, w.s)));
-    return join_shares<T>(part, p.rest_splits, rest, g.N, g.bias, out, w.s);
+    FFN_TRY((rows_of<T, AK, BK, EPI>(w, g, 0, p.shape, p.splits)));
+    g.M = M;
+    return rows_of<T, AK, BK, EPI>(w, g, p.main_rows, p.rest_shape, p.rest_splits);
 }
 template <class T>
 hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
-    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 512)), 0);
+    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 256)), false);
     g.rows_out = rows_out;
     if (p.splits > 1) g.part = (float*)w.take((size_t)p.splits * rows_out * g.N * 4);
     if (w.counting()) return hipSuccess;
@@ -646,13 +738,33 @@ hipError_t colsum(Work& w, const void* a, int64_t M, int64_t N, void* out) {
 // what the forward pass keeps: h planes, then p and q
 template <class T> inline size_t kept_h(int64_t M, int64_t H) { return up256(planes_bytes<T>(M, pad8(H))); }
 
+constexpr int FEW = 8;
+template <class T, int V, int MM, int RW>
+hipError_t few_go(const FfnArgs& f, T* h, hipStream_t s) {
+    const int64_t units = ((int64_t)f.H + RW / 2 - 1) / (RW / 2), outs = ((int64_t)f.O + RW / 2 - 1) / (RW / 2);
+    k_ffn_few<T, V, MM, RW, true><<<(unsigned)((units + 3) / 4), 256, 0, s>>>((const T*)f.x, (int)f.M, f.D, (const T*)f.w12, f.H, (const T*)f.b12, f.act, h);
+    k_ffn_few<T, V, MM, RW / 2, false><<<(unsigned)((outs + 3) / 4), 256, 0, s>>>(h, (int)f.M, f.H, (const T*)f.w3, f.O, (const T*)f.b3, f.act, (T*)f.y);
+    return hipGetLastError();
+}
+template <class T, int V>
+hipError_t few(const FfnArgs& f, T* h, hipStream_t s) {
+    return f.M == 1 ? few_go<T, V, 1, 2>(f, h, s) : f.M == 2 ? few_go<T, V, 2, 2>(f, h, s) : f.M <= 4 ? few_go<T, V, 4, 4>(f, h, s) : few_go<T, V, 8, 4>(f, h, s);
+}
+
 template <class T>
 hipError_t forward(const FfnArgs& f, Work& w) {
     const int64_t HP = pad8(f.H);
-    Operand x, w12, w3;
-    FFN_TRY(operand<T>(w, f.x, 1, f.M, f.D, x));
-    FFN_TRY(operand<T>(w, f.w12, 2, f.H, f.D, w12));
-    FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
+    if (f.M <= FEW && !f.kept) {
+        T* h = (T*)w.take((size_t)f.M * f.H * sizeof(T));
+        if (!w.counting()) {
+            constexpr int V = 16 / (int)sizeof(T);
+            const bool vec = f.D % V == 0 && f.H % V == 0 && aligned16(f.x) && aligned16(f.w12) && aligned16(f.w3);
+            return vec ? few<T, V>(f, h, w.s) : few<T, 1>(f, h, w.s);
+        }
+    }
+    Packer<T> pack(w);
+    const Operand x = pack.add(f.x, 1, f.M, f.D), w12 = pack.add(f.w12, 2, f.H, f.D), w3 = pack.add(f.w3, 1, f.O, f.H);
+    FFN_TRY(pack.go());
     char* h = (char*)f.kept;
     if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
     Prod g{};
@@ -671,36 +783,30 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     const bool all = w.counting(), hidden = all || f.dx || f.dw12 || f.db12;
     char* h = (char*)f.kept;
     const float* p = (const float*)(h + (all ? 0 : kept_h<T>(f.M, f.H)));
-    Operand dy{};
-    if (hidden || f.dw3) FFN_TRY(operand<T>(w, f.dy, 1, f.M, f.O, dy));
-    const int64_t GL = 2 * HP;
-    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, GL)) : nullptr, GL, f.M * GL};
+    Packer<T> pack(w);
+    Operand dy{}, w3{}, w12{}, x{};
+    if (hidden || f.dw3) dy = pack.add(f.dy, 1, f.M, f.O);
+    if (hidden) w3 = pack.add(f.w3, 1, f.O, f.H);
+    if (all || f.dx) w12 = pack.add(f.w12, 2, f.H, f.D);
+    if (all || f.dw12) x = pack.add(f.x, 1, f.M, f.D);
+    FFN_TRY(pack.go());
+    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
     if (hidden) {
-        Operand w3;
-        FFN_TRY(operand<T>(w, f.w3, 1, f.O, f.H, w3));
-        const int64_t slices = (f.M + 63) / 64;                       // (of 64 rows)
-        float* sums = all || f.db12 ? (float*)w.take((size_t)slices * 2 * f.H * 4) : nullptr;
-        {
-            Prod g{};
-            g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = GL;
-            g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
-            g.sums = sums;
-            FFN_TRY((product<T, KC, KS, EPI_DH>(w, g)));
-            if (!all && f.db12) FFN_TRY(join_columns<T>(sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
-        }
+        Prod g{};
+        g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = 2 * HP;
+        g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
+        const int slice = product_plan<T, EPI_DH>(g).shape == SHAPE_64 ? 32 : 64;
+        const int64_t slices = (f.M + slice - 1) / slice;
+        if (all || f.db12) g.sums = (float*)w.take((size_t)slices * 2 * f.H * 4);
+        FFN_TRY((product<T, KC, KS, EPI_DH>(w, g)));
+        if (!all && f.db12) FFN_TRY(join_columns<T>(g.sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
     }
     if (all || f.dx) {
-        Operand w12;
-        FFN_TRY(operand<T>(w, f.w12, 2, f.H, f.D, w12));
-        {
-            Prod g{};
-            g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
-            FFN_TRY((product<T, KC, KS, EPI_OUT>(w, g)));
-        }
+        Prod g{};
+        g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
+        FFN_TRY((product<T, KC, KS, EPI_OUT>(w, g)));
     }
     if (all || f.dw12) {
-        Operand x;
-        FFN_TRY(operand<T>(w, f.x, 1, f.M, f.D, x));
         Prod g{};
         g.a = dgu; g.b = x; g.M = 2 * HP; g.N = f.D; g.K = f.M; g.out = f.dw12; g.half_pad = HP; g.half = f.H;
         FFN_TRY(weight_gradient<T>(w, g, 2 * (int64_t)f.H));
