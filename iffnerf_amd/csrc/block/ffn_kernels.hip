@@ -137,7 +137,7 @@ struct Prod {
     // EPI_GATE: N = H; B rows n (gate) and up_row + n (up).  out = h planes of ld ldo; factors p, q [M][HP = pad8(H)] or null; bias b12
     // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
     // and with `sums`: [M / 32 MR][2H] column sums of dg and du (fp32, before they are rounded) over a wave's rows
-    int64_t up_row, HP, ldo; float* p; float* q; int act; float* sums;
+    int64_t up_row, HP, ldo, plane_o; float* p; float* q; int act; float* sums;
 };
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
@@ -165,8 +165,8 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
 
 // Tiles of 32 MR WM x 32 NR WN, 32 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
 // 1 KB per instruction, lane-linear in LDS) into a ring of NBUF buffers.  A KC tile is rows of 32 k
-// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 columns,
-// two rows per 256 bytes: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
+// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 and 192
+// columns, whose rows are not whole 256-byte bank rows: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
 // keep every LDS read free of bank conflicts.
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
 __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
     const E* const B = reinterpret_cast<const E*>(g.b.p);
 
     const auto swizzle = [](int r) { return KT == 64 ? (r >> 1) & 7 : (r >> 2) & 3; };
-    const auto turn = [](int r, int width) { return width == 64 ? (r & 2) << 1 : (r & 3) << 2; };
+    const auto turn = [](int r, int width) { return width % 128 ? (r & 2) << 1 : (r & 3) << 2; };
 
     // the lane's source of each piece, in bytes from the tile's corner at the step's k (ld < 2^22: 256 rows stay below 2^31), and its first k
     uint32_t oa[PA], ob[PB];
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
                 pv[i] = in ? uv * df : 0.0f;
                 v[i] = in ? f : 0.0f;
             }
-            store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.M * g.ldo, hv);
+            store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.plane_o, hv);
             if (g.p) {
                 Pack<float, 4>::store(g.p + m * g.HP + n, pv);
                 Pack<float, 4>::store(g.q + m * g.HP + n, v);
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
                 su[i] += q[i];
             }
             E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
-            store_planes<T>(o, g.M * g.ldo, p);
-            store_planes<T>(o + g.HP, g.M * g.ldo, q);
+            store_planes<T>(o, g.plane_o, p);
+            store_planes<T>(o + g.HP, g.plane_o, q);
         } else {
             int64_t row = m;
             if (!IN && g.half_pad) {
@@ -768,7 +768,7 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     char* h = (char*)f.kept;
     if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
     Prod g{};
-    g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.up_row = HP;
+    g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.plane_o = f.M * HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
     FFN_TRY((product<T, KC, KC, EPI_GATE>(w, g)));
     Prod d{};
@@ -793,7 +793,7 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
     if (hidden) {
         Prod g{};
-        g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = 2 * HP;
+        g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = 2 * HP; g.plane_o = dgu.plane;
         g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
         const int slice = product_plan<T, EPI_DH>(g).shape == SHAPE_64 ? 32 : 64;
         const int64_t slices = (f.M + slice - 1) / slice;

@@ -254,6 +254,17 @@ def test_gated_mlp(dev, M, D, H, O, act, bias, dtype):
     check_mlp(*make_mlp(M, D, H, O, dtype, bias, seed=M + D), act)
 
 
+# sizes at which each tile shape and each way of covering the rows is taken: whole 256 x 256 tiles, 256 x 192 ones in every layout, rows left to a
+# second launch (with and without shares of k), shares of a weight gradient, one round and several; one row more, one less
+@gpu
+@pytest.mark.parametrize("M,D,H,O,dtype", [
+    (16384 + 64, 1536, 256, 192, torch.bfloat16), (8192 + 40, 192, 1024, 1536, torch.bfloat16), (16384, 192, 2048, 384, torch.float16),
+    (4096 + 1, 768, 520, 768, torch.float16), (2048 + 255, 1536, 4096, 1536, torch.bfloat16), (4111, 384, 1023, 385, torch.float32),
+    (2049, 1536, 512, 1536, torch.float32), (8192 + 64, 128, 4096, 64, torch.bfloat16)])
+def test_gated_mlp_tile_shapes(dev, M, D, H, O, dtype):
+    check_mlp(*make_mlp(M, D, H, O, dtype, True, seed=M), "silu")
+
+
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_gated_mlp_layouts_and_partial_gradients(dev, dtype):
