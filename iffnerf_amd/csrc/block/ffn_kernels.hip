@@ -20,10 +20,10 @@ enum { ACT_SILU = 0, ACT_GELU = 1 };
 // act(g) and act'(g)
 template <bool EXACT>
 __device__ __forceinline__ void activation(int act, float g, float& f, float& df) {
-    if (act == ACT_SILU) {                         // s = 1 / (1 + e^-g), act = g s, act' = s (1 + g (1 - s))
-        const float s = 1.0f / (1.0f + (EXACT ? expf(-g) : __expf(-g)));
+    if (act == ACT_SILU) {                         // s = 1 / (1 + e^-g), act = g s, act' = s + g s (1 - s)
+        const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __builtin_amdgcn_rcpf(1.0f + __expf(-g));
         f = g * s;
-        df = s * fmaf(g, 1.0f - s, 1.0f);
+        df = fmaf(f, 1.0f - s, s);
     } else {                                       // c = (1 + erf(g / sqrt 2)) / 2, act = g c, act' = c + g e^(-g^2/2) / sqrt(2 pi)
         const float c = 0.5f * erfcf(-0.70710678118654752440f * g);
         f = g * c;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
     }
     float sg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool whole = m0 + BM <= g.M && n0 + NT <= g.N && !g.half_pad && (EPI != EPI_OUT || g.vec_out);
-    const auto slice = [&](int mb, int it, auto all_inside) {
+    const auto slice = [&](int mb, int it, auto all_inside, const float* pre) {
         constexpr bool IN = decltype(all_inside)::value;
         const int r = it * RPI + lane / CPL;
         if (64 % CPL && lane >= RPI * CPL) return;                    // (192 columns: 48 lanes work)
@@ -373,8 +373,13 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
         } else if constexpr (EPI == EPI_DH) {
             if (!IN && n >= g.HP) return;
             float p[4], q[4];
-            Pack<float, 4>::load(g.p + m * g.HP + n, p);
-            Pack<float, 4>::load(g.q + m * g.HP + n, q);
+            if (IN) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { p[i] = pre[i]; q[i] = pre[4 + i]; }
+            } else {
+                Pack<float, 4>::load(g.p + m * g.HP + n, p);
+                Pack<float, 4>::load(g.q + m * g.HP + n, q);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = IN || n + i < g.N;
@@ -413,6 +418,16 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
             }
         }
     };
+    float ahead[4][8];
+    const auto factors = [&](int mb, int it) {                        // p and q of four passes from pass `it` on
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = (m0 + wm + 32 * mb + (it + i) * RPI + lane / CPL) * g.HP + n;
+            Pack<float, 4>::load(g.p + at, ahead[i]);
+            Pack<float, 4>::load(g.q + at, ahead[i] + 4);
+        }
+    };
+    if (EPI == EPI_DH && whole) factors(0, 0);
     __syncthreads();                                                  // everybody has read the last fragments
 #pragma unroll
     for (int mb = 0; mb < MR; ++mb) {
@@ -422,13 +437,28 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
             for (int q4 = 0; q4 < 4; ++q4)
                 *reinterpret_cast<f32x4*>(tile + lr * OLD + 32 * nb + 8 * q4 + 4 * lh) =
                     f32x4{acc[nb][mb][4 * q4], acc[nb][mb][4 * q4 + 1], acc[nb][mb][4 * q4 + 2], acc[nb][mb][4 * q4 + 3]};
-        // a tile that lies wholly inside C: no checks between the passes, so that their reads and stores overlap
-        if (whole) {
+        // a tile that lies wholly inside C: no checks between the passes, so that their reads and stores overlap; the factors of the next
+        // passes are on their way while these are worked on
+        constexpr int ITS = 32 / RPI, GROUP = 4;
+        if (whole && EPI == EPI_DH) {
 #pragma unroll
-            for (int it = 0; it < 32 / RPI; ++it) slice(mb, it, std::true_type{});
+            for (int g0 = 0; g0 < ITS; g0 += GROUP) {
+                float now[GROUP][8];
+#pragma unroll
+                for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) now[i][j] = ahead[i][j];
+                const bool last = g0 + GROUP >= ITS;
+                if (!last || mb + 1 < MR) factors(last ? mb + 1 : mb, last ? 0 : g0 + GROUP);
+#pragma unroll
+                for (int i = 0; i < GROUP; ++i) slice(mb, g0 + i, std::true_type{}, now[i]);
+            }
+        } else if (whole) {
+#pragma unroll 4
+            for (int it = 0; it < ITS; ++it) slice(mb, it, std::true_type{}, nullptr);
         } else {
-#pragma unroll
-            for (int it = 0; it < 32 / RPI; ++it) slice(mb, it, std::false_type{});
+#pragma unroll 1
+            for (int it = 0; it < ITS; ++it) slice(mb, it, std::false_type{}, nullptr);
         }
     }
     if constexpr (EPI == EPI_DH) {
@@ -616,7 +646,7 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
 // ---- which tiles, and how many shares of the k loop.  A round is one tile on every CU (two of the 128 x 128 ones); its time is modelled as
 // the k loop at the rate measured on full rounds (1.8 us per 64 k of a 256 x 256 tile; the smaller tiles move more operand bytes per
 // product: 5 % and 20 % on top) plus the epilogue's traffic at 4.5 GB/ms.  Two things decide between the shapes: how full the last round is
-// (16 448 x 1536: 256 x 192 tiles are 2 rounds of 0.75, 256 x 256 ones 2 of 1 for 1.5 rounds of work), and the rows behind the last whole
+// (a weight gradient of 8192 x 1536: one round of 256 x 192 tiles in 369 us, 0.75 rounds of 256 x 256 ones in 447 us), and the rows behind the last whole
 // tile (257 tokens per image leave 64 of them): as tiles of 256 they can cost a whole round, as a second launch of 128 x 128 tiles
 // about 6 us and their k loop.
 // A product with few tiles is bound by the latency of its steps instead: 0.85 us per 64 k of a 128 x 128 tile alone on its CU with two buffers,
@@ -662,8 +692,8 @@ hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
     switch (shape) {
     case SHAPE_256: return tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s);
     case SHAPE_192:
-        if constexpr (EPI == EPI_OUT) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
-        return hipErrorInvalidConfiguration;
+        if constexpr (AK == KS) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
+        else return hipErrorInvalidConfiguration;
     case SHAPE_128: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
     case SHAPE_128_DEEP: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 4>(g, splits, s);
     default: return tiles<T, AK, BK, EPI, 2, 2, 1, 1, 64, 4>(g, splits, s);
@@ -691,7 +721,7 @@ Plan product_plan(const Prod& g) {
     constexpr double es = sizeof(T);
     const int64_t K = g.K * (Mat<T>::P == 3 ? 6 : 1);
     if (EPI == EPI_GATE) return plan_tiles(g.M, 2 * g.HP, K, (es + (g.p ? 8 : 0)) / 2, false, 1);
-    if (EPI == EPI_OUT) return plan_tiles(g.M, g.N, K, es, true, (int)std::max<int64_t>(1, std::min<int64_t>(16, g.K / 64)));
+    if (EPI == EPI_OUT) return plan_tiles(g.M, g.N, K, es, false, (int)std::max<int64_t>(1, std::min<int64_t>(16, g.K / 64)));
     Plan p = plan_tiles(g.M, g.HP, K, 8 + 2 * es, false, 1);
     if (p.rest_shape == SHAPE_64) p.rest_shape = SHAPE_128_DEEP;     // (one height of the waves' rows, that of the sums, per product)
     return p;
