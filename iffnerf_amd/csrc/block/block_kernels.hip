@@ -137,19 +137,37 @@ __global__ void __launch_bounds__(256) k_layernorm_bwd(const T* __restrict__ x, 
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
         for (int i = 0; i < V; ++i) aw[c][i] = ab[c][i] = 0.0f;
-    for (uint32_t row = blockIdx.x * RPB + (WPR == 1 ? wave : 0); row < M; row += gridDim.x * RPB) {
-        const T* xr = x + xv.at(row);
-        const T* gr = dy + (int64_t)row * D;
-        const float2 st = stats[row];
+    // the next row's values are on their way while this one is reduced (raw: half the registers of a 16-bit type's fp32 values)
+    typename Raw<T, V>::t rx[NCH], rg[NCH];
+    float2 nst = make_float2(0.0f, 0.0f);
+    const auto fetch = [&](uint32_t r) {
+        const T* xr = x + xv.at(r);
+        const T* gr = dy + (int64_t)r * D;
+        nst = stats[r];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = (c * TPR + t) * V;
+            if (col < D) {
+                rx[c] = *reinterpret_cast<const typename Raw<T, V>::t*>(xr + col);
+                rg[c] = *reinterpret_cast<const typename Raw<T, V>::t*>(gr + col);
+            }
+        }
+    };
+    uint32_t row = blockIdx.x * RPB + (WPR == 1 ? wave : 0);
+    if (row < M) fetch(row);
+    for (; row < M; row += gridDim.x * RPB) {
+        const float2 st = nst;
         float xh[NCH][V], e[NCH][V];
         float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            if ((c * TPR + t) * V < D) { Raw<T, V>::unpack(rx[c], xh[c]); Raw<T, V>::unpack(rg[c], e[c]); }
+        if (row + gridDim.x * RPB < M) fetch(row + gridDim.x * RPB);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const int col = (c * TPR + t) * V;
             if (col < D) {
                 float g[V];
-                Pack<T, V>::load(xr + col, xh[c]);
-                Pack<T, V>::load(gr + col, e[c]);
                 load_par<T, V>(w, wk, col, g, 1.0f);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -248,22 +266,24 @@ __device__ __forceinline__ void put_par(void* p, int kind, int64_t c, float v) {
     if (kind == W_F32) reinterpret_cast<float*>(p)[c] = v;
     else reinterpret_cast<T*>(p)[c] = (T)v;
 }
-// dw[c], db[c] = sum over the G shares: 16 columns x 16 groups of shares per workgroup, groups joined in order
+// dw[c], db[c] = sum over the G shares: 16 columns x 64 groups of shares per workgroup, groups joined in order (a thread then waits for
+// G / 64 loads: 11 us with 16 groups of 512 shares, 5 with 64)
 template <class T>
-__global__ void __launch_bounds__(256) k_layernorm_params(const float* __restrict__ part, int G, int D, void* __restrict__ dw,
-                                                          void* __restrict__ db, int kind) {
-    __shared__ float s[16][17];
+__global__ void __launch_bounds__(1024) k_layernorm_params(const float* __restrict__ part, int G, int D, void* __restrict__ dw,
+                                                           void* __restrict__ db, int kind) {
+    __shared__ float s[64][17];
     const int c16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
     const int64_t c = blockIdx.x * (int64_t)16 + c16;          // over dw's columns, then db's
     const int64_t W = 2 * (int64_t)D;
     float a = 0.0f;
     if (c < W)
-        for (int g = grp; g < G; g += 16) a += part[g * W + c];
+#pragma unroll 8
+        for (int g = grp; g < G; g += 64) a += part[g * W + c];
     s[grp][c16] = a;
     __syncthreads();
     if (grp == 0 && c < W) {
         float v = s[0][c16];
-        for (int j = 1; j < 16; ++j) v += s[j][c16];
+        for (int j = 1; j < 64; ++j) v += s[j][c16];
         if (c < D) { if (dw) put_par<T>(dw, kind, c, v); }
         else if (db) put_par<T>(db, kind, c - D, v);
     }
@@ -396,7 +416,7 @@ hipError_t norm_bwd(const NormArgs& a, float* part, hipStream_t s) {
         }
     }
     if (params)
-        k_layernorm_params<T><<<(int)((2 * (int64_t)a.D + 15) / 16), 256, 0, s>>>(part, a.rows ? G : 0, a.D, a.dw, a.db, a.dwk);
+        k_layernorm_params<T><<<(int)((2 * (int64_t)a.D + 15) / 16), 1024, 0, s>>>(part, a.rows ? G : 0, a.D, a.dw, a.db, a.dwk);
     return hipGetLastError();
 }
 
@@ -414,7 +434,8 @@ hipError_t dropout_go(const void* x, const void* res, void* y, int64_t n, uint32
 
 }  // namespace
 
-int norm_bwd_groups(uint32_t rows) { return (int)std::min<uint32_t>((rows + 3) / 4, 512); }
+// four workgroups per CU (65 792 x 1024 bf16: 82 us, 91 with two), each with at least 8 rows (3724 x 1001 fp16: 17 us with 512, 22 with 1024)
+int norm_bwd_groups(uint32_t rows) { return (int)std::min<uint32_t>((rows + 7) / 8, 1024); }
 
 hipError_t launch_layernorm_fwd(const NormArgs& a, hipStream_t s) {
     if (!a.rows || !a.D) return hipSuccess;

@@ -44,6 +44,26 @@ template <class T, class T8> struct Pack8 {
 template <> struct Pack<__bf16, 8> : Pack8<__bf16, bf16x8> {};
 template <> struct Pack<_Float16, 8> : Pack8<_Float16, f16x8> {};
 
+// the same V elements as they are in memory
+template <class T, int V> struct Raw;
+template <class T> struct Raw<T, 1> {
+    typedef T t;
+    static __device__ __forceinline__ void unpack(T r, float v[1]) { v[0] = (float)r; }
+};
+template <> struct Raw<float, 4> {
+    typedef f32x4 t;
+    static __device__ __forceinline__ void unpack(f32x4 r, float v[4]) { v[0] = r[0]; v[1] = r[1]; v[2] = r[2]; v[3] = r[3]; }
+};
+template <class T8> struct Raw8 {
+    typedef T8 t;
+    static __device__ __forceinline__ void unpack(T8 r, float v[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)r[i];
+    }
+};
+template <> struct Raw<__bf16, 8> : Raw8<bf16x8> {};
+template <> struct Raw<_Float16, 8> : Raw8<f16x8> {};
+
 inline size_t dt_size(int dt) { return dt == IFF_DT_F32 ? 4 : 2; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

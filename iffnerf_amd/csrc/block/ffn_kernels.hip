@@ -548,20 +548,20 @@ __global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part
     }
 }
 
-// out[c] = sum_g part[g][c]: 16 columns x 16 groups of shares per workgroup, groups joined in order
+// out[c] = sum_g part[g][c]: 16 columns x 64 groups of shares per workgroup, groups joined in order
 template <class T>
-__global__ void __launch_bounds__(256) k_ffn_join_columns(const float* __restrict__ part, int64_t G, int64_t N, T* __restrict__ out) {
-    __shared__ float s[16][17];
+__global__ void __launch_bounds__(1024) k_ffn_join_columns(const float* __restrict__ part, int64_t G, int64_t N, T* __restrict__ out) {
+    __shared__ float s[64][17];
     const int c16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
     const int64_t c = blockIdx.x * (int64_t)16 + c16;
     float a = 0.0f;
     if (c < N)
 #pragma unroll 8
-        for (int64_t g = grp; g < G; g += 16) a += part[g * N + c];
+        for (int64_t g = grp; g < G; g += 64) a += part[g * N + c];
     s[grp][c16] = a;
     __syncthreads();
     if (grp == 0 && c < N) {
-        for (int j = 1; j < 16; ++j) a += s[j][c16];
+        for (int j = 1; j < 64; ++j) a += s[j][c16];
         out[c] = (T)a;
     }
 }
@@ -669,7 +669,7 @@ inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool m
     double least = 1e300, rest = 1e300;
     const int64_t whole = may_rest ? M / 256 * 256 : 0;
     int rest_shape = SHAPE_128, rest_splits = 1;
-    for (int z = 1; z <= most && (z == 1 || K / z >= 256); ++z)
+    for (int z = 1; z <= most && (z == 1 || K / z >= 256); z += z < 8 ? 1 : z < 16 ? 2 : 8)      // (1 .. 8, 10 .. 16, 24 .. 64: this runs at every call)
         for (int shape = SHAPE_256; shape < SHAPES; ++shape) {
             if (shape == SHAPE_192 && !may_192) continue;
             const double all = round_time(shape, M, N, K, z, out_bytes) + share_time(M, N, z);
@@ -748,7 +748,7 @@ hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
 }
 template <class T>
 hipError_t join_columns(const float* part, int64_t G, int64_t N, void* out, hipStream_t s) {
-    k_ffn_join_columns<T><<<(unsigned)((N + 15) / 16), 256, 0, s>>>(part, G, N, (T*)out);
+    k_ffn_join_columns<T><<<(unsigned)((N + 15) / 16), 1024, 0, s>>>(part, G, N, (T*)out);
     return hipGetLastError();
 }
 // shares: enough workgroups for the chip, each at least 64 rows

@@ -9,6 +9,7 @@ the tensors' device, allocate through torch (so they can be captured into a hipG
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Union
 
@@ -35,6 +36,12 @@ def _run(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(i))
     if rc:
         check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(name: str, *sizes) -> int:
+    """What the size query ``name`` of the library answers (a function of the sizes alone)."""
+    return int(getattr(_lib.lib(), name)(*sizes))
 
 
 def _first_derivative(backward):
@@ -119,7 +126,7 @@ class _LayerNorm(torch.autograd.Function):
         db = x.new_empty((D,), dtype=par) if need_b else None
         nbytes, ws = 0, None
         if need_w or need_b:
-            nbytes = _lib._lib.iff_layer_norm_backward_workspace(n0 * n1, D)
+            nbytes = _bytes("iff_layer_norm_backward_workspace", n0 * n1, D)
             ws = _workspace(nbytes, x)
         _run("iff_layer_norm_backward", x.device, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _TYPES[par],
              stats.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
@@ -159,10 +166,9 @@ def _mlp_forward(x, w12, b12, w3, b3, act, keep):
     M, D = x.shape
     O, H = w3.shape
     ty = _TYPES[x.dtype]
-    L = _lib._lib or _lib.lib()
     y = x.new_empty((M, O))
-    kept = x.new_empty((L.iff_gated_mlp_kept_bytes(ty, M, D, H, O),), dtype=torch.uint8) if keep else None
-    ws = _workspace(L.iff_gated_mlp_forward_workspace(ty, M, D, H, O), x)
+    kept = x.new_empty((_bytes("iff_gated_mlp_kept_bytes", ty, M, D, H, O),), dtype=torch.uint8) if keep else None
+    ws = _workspace(_bytes("iff_gated_mlp_forward_workspace", ty, M, D, H, O), x)
     _run("iff_gated_mlp_forward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), _ptr(b12), w3.data_ptr(), _ptr(b3), act, y.data_ptr(),
          _ptr(kept), kept.numel() if keep else 0, ws.data_ptr(), ws.numel())
     return y, kept
@@ -188,7 +194,7 @@ class _GatedMlp(torch.autograd.Function):
         db12 = x.new_empty((2 * H,)) if need[2] else None
         dw3 = x.new_empty((O, H)) if need[3] else None
         db3 = x.new_empty((O,)) if need[4] else None
-        ws = _workspace(_lib._lib.iff_gated_mlp_backward_workspace(ty, M, D, H, O), x)
+        ws = _workspace(_bytes("iff_gated_mlp_backward_workspace", ty, M, D, H, O), x)
         _run("iff_gated_mlp_backward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), kept.data_ptr(),
              dy.data_ptr(), _ptr(dx), _ptr(dw12), _ptr(db12), _ptr(dw3), _ptr(db3), ws.data_ptr(), ws.numel())
         return dx, dw12, db12, dw3, db3, None
