@@ -479,10 +479,12 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
 // ------------------------------------------------------------------------------------------------ a few tokens
 // At most 8 rows and no gradients (serving token by token): the weights are read once and that is all the time there is, so the products are
 // vector dot products -- a wave per RW rows of the weight matrix, its lanes over k, 16 bytes per load, fp32 sums joined across the lanes --
-// and not tiles of which 8 of 128 rows would be used.  GATE: RW / 2 hidden units, their gate and their up row; else RW outputs.
-template <class T, int V, int MM, int RW, bool GATE>
-__global__ void __launch_bounds__(256) k_ffn_few(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, int64_t N, const T* __restrict__ bias,
-                                                 int act, T* __restrict__ out) {
+// and not tiles of which 8 of 128 rows would be used.  GATE: RW / 2 hidden units, their gate and their up row; else RW outputs.  The hidden
+// activation stays fp32 between the two launches.  One token, 1536 x 4096 bf16: 5.9 + 4.2 us, 3.7 TB/s of weights.
+template <class T, int V, int MM, int RW, bool GATE, class TX, class TO>
+__global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M, int64_t K, const T* __restrict__ w, int64_t N, const T* __restrict__ bias,
+                                                 int act, TO* __restrict__ out) {
+    constexpr int VX = V == 1 ? 1 : 16 / (int)sizeof(TX) < V ? 16 / (int)sizeof(TX) : V;
     constexpr int U = GATE ? RW / 2 : RW;                            // columns of the output per wave
     const int lane = threadIdx.x & 63;
     const int64_t n0 = (blockIdx.x * (int64_t)4 + (threadIdx.x >> 6)) * U;
@@ -506,7 +508,8 @@ __global__ void __launch_bounds__(256) k_ffn_few(const T* __restrict__ x, int M,
 #pragma unroll
         for (int m = 0; m < MM; ++m) {
             float b[V];
-            Pack<T, V>::load(x + min(m, M - 1) * K + k, b);
+#pragma unroll
+            for (int i = 0; i < V; i += VX) Pack<TX, VX>::load(x + min(m, M - 1) * K + k + i, b + i);
 #pragma unroll
             for (int r = 0; r < RW; ++r)
 #pragma unroll
@@ -533,7 +536,7 @@ __global__ void __launch_bounds__(256) k_ffn_few(const T* __restrict__ x, int M,
                 activation<Mat<T>::P == 3>(act, v, f, df);
                 v = f * up;
             }
-            out[m * N + n] = (T)v;
+            out[m * N + n] = (TO)v;
         }
 }
 
@@ -770,14 +773,14 @@ template <class T> inline size_t kept_h(int64_t M, int64_t H) { return up256(pla
 
 constexpr int FEW = 8;
 template <class T, int V, int MM, int RW>
-hipError_t few_go(const FfnArgs& f, T* h, hipStream_t s) {
+hipError_t few_go(const FfnArgs& f, float* h, hipStream_t s) {
     const int64_t units = ((int64_t)f.H + RW / 2 - 1) / (RW / 2), outs = ((int64_t)f.O + RW / 2 - 1) / (RW / 2);
-    k_ffn_few<T, V, MM, RW, true><<<(unsigned)((units + 3) / 4), 256, 0, s>>>((const T*)f.x, (int)f.M, f.D, (const T*)f.w12, f.H, (const T*)f.b12, f.act, h);
-    k_ffn_few<T, V, MM, RW / 2, false><<<(unsigned)((outs + 3) / 4), 256, 0, s>>>(h, (int)f.M, f.H, (const T*)f.w3, f.O, (const T*)f.b3, f.act, (T*)f.y);
+    k_ffn_few<T, V, MM, RW, true, T, float><<<(unsigned)((units + 3) / 4), 256, 0, s>>>((const T*)f.x, (int)f.M, f.D, (const T*)f.w12, f.H, (const T*)f.b12, f.act, h);
+    k_ffn_few<T, V, MM, RW / 2, false, float, T><<<(unsigned)((outs + 3) / 4), 256, 0, s>>>(h, (int)f.M, f.H, (const T*)f.w3, f.O, (const T*)f.b3, f.act, (T*)f.y);
     return hipGetLastError();
 }
 template <class T, int V>
-hipError_t few(const FfnArgs& f, T* h, hipStream_t s) {
+hipError_t few(const FfnArgs& f, float* h, hipStream_t s) {
     return f.M == 1 ? few_go<T, V, 1, 2>(f, h, s) : f.M == 2 ? few_go<T, V, 2, 2>(f, h, s) : f.M <= 4 ? few_go<T, V, 4, 4>(f, h, s) : few_go<T, V, 8, 4>(f, h, s);
 }
 
@@ -785,7 +788,7 @@ template <class T>
 hipError_t forward(const FfnArgs& f, Work& w) {
     const int64_t HP = pad8(f.H);
     if (f.M <= FEW && !f.kept) {
-        T* h = (T*)w.take((size_t)f.M * f.H * sizeof(T));
+        float* h = (float*)w.take((size_t)f.M * f.H * 4);
         if (!w.counting()) {
             constexpr int V = 16 / (int)sizeof(T);
             const bool vec = f.D % V == 0 && f.H % V == 0 && aligned16(f.x) && aligned16(f.w12) && aligned16(f.w3);
