@@ -26,13 +26,12 @@ static int fail(int code, const char* fmt, ...) {
     } while (0)
 
 static bool block_type(int32_t t) { return t == IFF_TYPE_F32 || t == IFF_TYPE_BF16 || t == IFF_TYPE_F16; }
-static int64_t block_limit() { return (int64_t)1 << 30; }
 
 static int check_norm(const char* who, int32_t x_type, int64_t n0, int64_t n1, int32_t width, int32_t par_type) {
     IFF_REQUIRE(block_type(x_type), "%s: type %d is not one of IFF_TYPE_F32 / BF16 / F16", who, x_type);
     IFF_REQUIRE(par_type == IFF_TYPE_F32 || par_type == x_type, "%s: parameters of type %d with activations of type %d (fp32 or the same)", who, par_type, x_type);
     IFF_REQUIRE(n0 >= 0 && n1 >= 0 && (n1 == 0 || n0 <= INT32_MAX / n1), "%s: bad row counts %lld x %lld", who, (long long)n0, (long long)n1);
-    IFF_REQUIRE(width >= 1 && width <= block_limit(), "%s: bad width %d", who, width);
+    IFF_REQUIRE(width >= 1 && width <= (1 << 24), "%s: bad width %d", who, width);
     return 0;
 }
 static NormArgs norm_args(const void* x, int32_t x_type, int64_t n0, int64_t n1, int64_t stride0, int64_t stride1, int32_t width, const void* w,
@@ -48,6 +47,7 @@ extern "C" int iff_layer_norm_forward(const void* x, int32_t x_type, int64_t n0,
     IFF_REQUIRE(eps >= 0.0f, "iff_layer_norm_forward: eps must not be negative");
     if (n0 * n1 == 0) return 0;
     IFF_REQUIRE(x && y, "iff_layer_norm_forward: null buffer");
+    IFF_REQUIRE(((uintptr_t)stats_opt & 7) == 0, "iff_layer_norm_forward: stats must be 8-byte aligned");
     NormArgs a = norm_args(x, x_type, n0, n1, stride0, stride1, width, w_opt, par_type);
     a.b = b_opt; a.bk = !b_opt ? 0 : par_type == IFF_TYPE_F32 ? 1 : 2;
     a.eps = eps; a.y = y; a.stats = stats_opt;
@@ -65,6 +65,7 @@ extern "C" int iff_layer_norm_backward(const void* x, int32_t x_type, int64_t n0
     const int64_t rows = n0 * n1;
     if (!dx_opt && !dw_opt && !db_opt) return 0;
     IFF_REQUIRE(rows == 0 || (x && stats && dy), "iff_layer_norm_backward: null buffer");
+    IFF_REQUIRE(((uintptr_t)stats & 7) == 0, "iff_layer_norm_backward: stats must be 8-byte aligned");
     const bool params = dw_opt || db_opt;
     const size_t need = params ? iff_layer_norm_backward_workspace(rows, width) : 0;
     if (need && (!workspace || workspace_bytes < need))

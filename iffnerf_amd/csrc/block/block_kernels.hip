@@ -62,64 +62,66 @@ __global__ void __launch_bounds__(256) k_layernorm_fwd(const T* __restrict__ x, 
     constexpr int TPR = 64 * WPR;
     __shared__ float s[4];
     const int t = threadIdx.x % TPR;
-    const uint32_t row = WPR == 1 ? blockIdx.x * 4u + (threadIdx.x >> 6) : blockIdx.x;
-    if (row >= M) return;
-    const T* xr = x + xv.at(row);
-    float v[NCH][V];
-    float sum = 0.0f;
+    constexpr uint32_t RPB = 4 / WPR;
+    for (uint32_t row = blockIdx.x * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0); row < M; row += gridDim.x * RPB) {
+        const T* xr = x + xv.at(row);
+        float v[NCH][V];
+        float sum = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int col = (c * TPR + t) * V;
-        if (col < D) Pack<T, V>::load(xr + col, v[c]);
-        else
+        for (int c = 0; c < NCH; ++c) {
+            const int col = (c * TPR + t) * V;
+            if (col < D) Pack<T, V>::load(xr + col, v[c]);
+            else
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[c][i] = 0.0f;
+                for (int i = 0; i < V; ++i) v[c][i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum += v[c][i];
-    }
-    const float mean = row_sum<WPR>(sum, s) / (float)D;
-    float sq = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c)
-        if ((c * TPR + t) * V < D) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) { const float d = v[c][i] - mean; sq = fmaf(d, d, sq); }
+            for (int i = 0; i < V; ++i) sum += v[c][i];
         }
-    const float r = 1.0f / sqrtf(row_sum<WPR>(sq, s) / (float)D + eps);
+        const float mean = row_sum<WPR>(sum, s) / (float)D;
+        float sq = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int col = (c * TPR + t) * V;
-        if (col >= D) continue;
-        float g[V], h[V], o[V];
-        load_par<T, V>(w, wk, col, g, 1.0f);
-        load_par<T, V>(b, bk, col, h, 0.0f);
+        for (int c = 0; c < NCH; ++c)
+            if ((c * TPR + t) * V < D) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = fmaf((v[c][i] - mean) * r, g[i], h[i]);
-        Pack<T, V>::store(y + (int64_t)row * D + col, o);
+                for (int i = 0; i < V; ++i) { const float d = v[c][i] - mean; sq = fmaf(d, d, sq); }
+            }
+        const float r = 1.0f / sqrtf(row_sum<WPR>(sq, s) / (float)D + eps);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = (c * TPR + t) * V;
+            if (col >= D) continue;
+            float g[V], h[V], o[V];
+            load_par<T, V>(w, wk, col, g, 1.0f);
+            load_par<T, V>(b, bk, col, h, 0.0f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = fmaf((v[c][i] - mean) * r, g[i], h[i]);
+            Pack<T, V>::store(y + (int64_t)row * D + col, o);
+        }
+        if (stats && t == 0) stats[row] = make_float2(mean, r);
     }
-    if (stats && t == 0) stats[row] = make_float2(mean, r);
 }
 
 // rows of any width: one workgroup per row, the row read three times (from the L2 after the first)
 template <class T>
-__global__ void __launch_bounds__(256) k_layernorm_fwd_any(const T* __restrict__ x, RowView xv, int D, const void* __restrict__ w,
+__global__ void __launch_bounds__(256) k_layernorm_fwd_any(const T* __restrict__ x, RowView xv, uint32_t M, int D, const void* __restrict__ w,
                                                            const void* __restrict__ b, int wk, int bk, float eps, T* __restrict__ y,
                                                            float2* __restrict__ stats) {
     __shared__ float s[4];
-    const uint32_t row = blockIdx.x;
-    const T* xr = x + xv.at(row);
-    float sum = 0.0f, sq = 0.0f;
-    for (int c = threadIdx.x; c < D; c += 256) sum += (float)xr[c];
-    const float mean = row_sum<4>(sum, s) / (float)D;
-    for (int c = threadIdx.x; c < D; c += 256) { const float d = (float)xr[c] - mean; sq = fmaf(d, d, sq); }
-    const float r = 1.0f / sqrtf(row_sum<4>(sq, s) / (float)D + eps);
-    for (int c = threadIdx.x; c < D; c += 256) {
-        float g[1], h[1];
-        load_par<T, 1>(w, wk, c, g, 1.0f);
-        load_par<T, 1>(b, bk, c, h, 0.0f);
-        y[(int64_t)row * D + c] = (T)fmaf(((float)xr[c] - mean) * r, g[0], h[0]);
+    for (uint32_t row = blockIdx.x; row < M; row += gridDim.x) {
+        const T* xr = x + xv.at(row);
+        float sum = 0.0f, sq = 0.0f;
+        for (int c = threadIdx.x; c < D; c += 256) sum += (float)xr[c];
+        const float mean = row_sum<4>(sum, s) / (float)D;
+        for (int c = threadIdx.x; c < D; c += 256) { const float d = (float)xr[c] - mean; sq = fmaf(d, d, sq); }
+        const float r = 1.0f / sqrtf(row_sum<4>(sq, s) / (float)D + eps);
+        for (int c = threadIdx.x; c < D; c += 256) {
+            float g[1], h[1];
+            load_par<T, 1>(w, wk, c, g, 1.0f);
+            load_par<T, 1>(b, bk, c, h, 0.0f);
+            y[(int64_t)row * D + c] = (T)fmaf(((float)xr[c] - mean) * r, g[0], h[0]);
+        }
+        if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, r);
     }
-    if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, r);
 }
 
 // dx of the rows a workgroup takes (every gridDim-th), and its share of dw / db: part[blockIdx][0] = sum dy xh, [1] = sum dy over its
@@ -220,28 +222,29 @@ __global__ void __launch_bounds__(256) k_layernorm_bwd(const T* __restrict__ x, 
 
 // any width: dx one workgroup per row
 template <class T>
-__global__ void __launch_bounds__(256) k_layernorm_dx_any(const T* __restrict__ x, RowView xv, const T* __restrict__ dy, int D,
+__global__ void __launch_bounds__(256) k_layernorm_dx_any(const T* __restrict__ x, RowView xv, const T* __restrict__ dy, uint32_t M, int D,
                                                           const void* __restrict__ w, int wk, const float2* __restrict__ stats,
                                                           T* __restrict__ dx) {
     __shared__ float s[4];
-    const uint32_t row = blockIdx.x;
-    const T* xr = x + xv.at(row);
-    const T* gr = dy + (int64_t)row * D;
-    const float2 st = stats[row];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < D; c += 256) {
-        float g[1];
-        load_par<T, 1>(w, wk, c, g, 1.0f);
-        const float e = (float)gr[c] * g[0];
-        s1 += e;
-        s2 = fmaf(e, ((float)xr[c] - st.x) * st.y, s2);
-    }
-    const float m1 = row_sum<4>(s1, s) / (float)D, m2 = row_sum<4>(s2, s) / (float)D;
-    for (int c = threadIdx.x; c < D; c += 256) {
-        float g[1];
-        load_par<T, 1>(w, wk, c, g, 1.0f);
-        const float xh = ((float)xr[c] - st.x) * st.y;
-        dx[(int64_t)row * D + c] = (T)(st.y * ((float)gr[c] * g[0] - m1 - xh * m2));
+    for (uint32_t row = blockIdx.x; row < M; row += gridDim.x) {
+        const T* xr = x + xv.at(row);
+        const T* gr = dy + (int64_t)row * D;
+        const float2 st = stats[row];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int c = threadIdx.x; c < D; c += 256) {
+            float g[1];
+            load_par<T, 1>(w, wk, c, g, 1.0f);
+            const float e = (float)gr[c] * g[0];
+            s1 += e;
+            s2 = fmaf(e, ((float)xr[c] - st.x) * st.y, s2);
+        }
+        const float m1 = row_sum<4>(s1, s) / (float)D, m2 = row_sum<4>(s2, s) / (float)D;
+        for (int c = threadIdx.x; c < D; c += 256) {
+            float g[1];
+            load_par<T, 1>(w, wk, c, g, 1.0f);
+            const float xh = ((float)xr[c] - st.x) * st.y;
+            dx[(int64_t)row * D + c] = (T)(st.y * ((float)gr[c] * g[0] - m1 - xh * m2));
+        }
     }
 }
 // any width: the shares of dw / db, a thread per column, the rows of block y in increasing order
@@ -359,9 +362,11 @@ inline NormShape norm_shape(int dt, int D, bool aligned) {
     return {false, 4, 0};
 }
 
+inline uint32_t norm_grid(uint32_t wgs) { return std::min<uint32_t>(wgs, 1u << 22); }      // (a launch has fewer than 2^32 threads)
+
 template <class T, int V, int NCH, int WPR>
 void fwd_go(const NormArgs& a, RowView xv, hipStream_t s) {
-    k_layernorm_fwd<T, V, NCH, WPR><<<WPR == 1 ? (a.rows + 3) / 4 : a.rows, 256, 0, s>>>((const T*)a.x, xv, a.rows, a.D, a.w, a.b, a.wk, a.bk, a.eps,
+    k_layernorm_fwd<T, V, NCH, WPR><<<norm_grid(WPR == 1 ? (a.rows + 3) / 4 : a.rows), 256, 0, s>>>((const T*)a.x, xv, a.rows, a.D, a.w, a.b, a.wk, a.bk, a.eps,
                                                                                      (T*)a.y, (float2*)a.stats);
 }
 template <class T, int V, int NCH, int WPR>
@@ -387,7 +392,7 @@ hipError_t norm_fwd(const NormArgs& a, hipStream_t s) {
     const int V = 16 / (int)sizeof(T);
     const bool al = aligned16(a.x) && aligned16(a.y) && aligned16(a.w) && aligned16(a.b) && a.s0 % V == 0 && a.s1 % V == 0;
     const NormShape sh = norm_shape(a.dt, a.D, al);
-    if (!sh.nch) k_layernorm_fwd_any<T><<<a.rows, 256, 0, s>>>((const T*)a.x, xv, a.D, a.w, a.b, a.wk, a.bk, a.eps, (T*)a.y, (float2*)a.stats);
+    if (!sh.nch) k_layernorm_fwd_any<T><<<norm_grid(a.rows), 256, 0, s>>>((const T*)a.x, xv, a.rows, a.D, a.w, a.b, a.wk, a.bk, a.eps, (T*)a.y, (float2*)a.stats);
     else {
 #define GO(v, n, p) fwd_go<T, v, n, p>(a, xv, s)
         NORM_FORMS(T, sh, GO);
@@ -405,7 +410,7 @@ hipError_t norm_bwd(const NormArgs& a, float* part, hipStream_t s) {
     const int G = norm_bwd_groups(a.rows);
     if (a.rows) {
         if (!sh.nch) {
-            if (a.dx) k_layernorm_dx_any<T><<<a.rows, 256, 0, s>>>((const T*)a.x, xv, (const T*)a.dy, a.D, a.w, a.wk, (const float2*)a.stats, (T*)a.dx);
+            if (a.dx) k_layernorm_dx_any<T><<<norm_grid(a.rows), 256, 0, s>>>((const T*)a.x, xv, (const T*)a.dy, a.rows, a.D, a.w, a.wk, (const float2*)a.stats, (T*)a.dx);
             if (params)
                 k_layernorm_part_any<T><<<dim3((a.D + 255) / 256, G), 256, 0, s>>>((const T*)a.x, xv, (const T*)a.dy, a.rows, a.D,
                                                                                    (const float2*)a.stats, part);

@@ -641,7 +641,7 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
     constexpr int BM = 32 * MR * WM, NT = EPI == EPI_GATE ? 16 * NR * WN : 32 * NR * WN;
     const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M - g.m_base + BM - 1) / BM, gn = (N + NT - 1) / NT;
     if (gm <= 0 || !gn) return hipSuccess;
-    if (gm * gn > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    if (gm * gn >= (1ll << 32) / (64 * WM * WN)) return hipErrorInvalidConfiguration;      // (a launch has fewer than 2^32 threads)
     g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 63) / 64 * 64 : std::max<int64_t>(g.K, 64);
     k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, KT, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
     return hipGetLastError();

@@ -543,8 +543,8 @@ int iff_pose_errors(const float* c2w, const float* gt_c2w, const float* parts_op
 /* ------------------------------------------------------------------------------------------------ trainable block operators
  * The feed-forward half of a pre-norm transformer block, x + dropout(gated_mlp(layer_norm(x))), WITH its gradients: what fine-tuning the
  * image backbone (pose_estimation/backbone.py:12-14) inside pose_estimation/train.py:97-119 runs per block.  Tensors are fp32, bf16 or
- * fp16 (IFF_TYPE_*), arithmetic and every sum fp32; results are rounded to the tensors' type once.  Row counts are below 2^31, widths
- * below 2^30; empty tensors are no-ops (gradients of parameters over no rows are zero).  Calls are reproducible bit for bit: no atomics. */
+ * fp16 (IFF_TYPE_*), arithmetic and every sum fp32; results are rounded to the tensors' type once.  Row counts are below 2^31, a
+ * norm's width is at most 2^24; pointers are aligned to their element (statistics to 8 bytes) and outputs overlap no input; empty tensors are no-ops (gradients of parameters over no rows are zero).  Calls are reproducible bit for bit: no atomics. */
 #define IFF_TYPE_F32  0
 #define IFF_TYPE_BF16 1
 #define IFF_TYPE_F16  2

@@ -395,6 +395,43 @@ def test_dropout_layouts_and_values(dev):
 
 
 @gpu
+def test_offsets_past_32_bits(dev):
+    """Tensors of more than 2^31 elements (2^32 bytes and more): the last values against small calls on the same values."""
+    n = 2 ** 31 + 13
+    y = hip_block.dropout(torch.ones(n, dtype=torch.bfloat16, device=dev), 0.5, 11)
+    last = (n - 1) // 8
+    bits = []
+    c, k = [last, 0, 0, 0], [11, 0]
+    for _ in range(10):
+        p0, p1 = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(p1 >> 32) ^ c[1] ^ k[0], p1 & 0xFFFFFFFF, (p0 >> 32) ^ c[3] ^ k[1], p0 & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    for w in c:
+        bits += [w & 0xFFFF, w >> 16]
+    assert y[last * 8:].tolist() == [2.0 if b >= 32768 else 0.0 for b in bits[:n - last * 8]]
+    del y
+    base = torch.zeros(2 ** 32 + 128, dtype=torch.float16, device=dev)
+    x = base.as_strided((2, 64), (2 ** 32 + 64, 1))
+    x.copy_(normal((2, 64), 60, torch.float16))
+    assert torch.equal(hip_block.layer_norm(x), hip_block.layer_norm(x.contiguous()))
+    del base, x
+    M, D, H = 2 ** 20 + 300, 2048, 8
+    x = torch.zeros(M, D, dtype=torch.bfloat16, device=dev)
+    tail = normal((300, D), 61, torch.bfloat16)
+    x[-300:] = tail
+    _, w12, b12, w3, b3, _ = make_mlp(1, D, H, 8, torch.bfloat16, True, seed=62)
+    small, large = tail.requires_grad_(True), x.requires_grad_(True)
+    dy = normal((300, 8), 63, torch.bfloat16)
+    ys, yl = hip_block.gated_mlp(small, w12, b12, w3, b3), hip_block.gated_mlp(large, w12, b12, w3, b3)
+    gs = torch.autograd.grad(ys, small, dy)[0]
+    gl = torch.autograd.grad(yl, large, torch.cat((torch.zeros(M - 300, 8, dtype=torch.bfloat16, device=dev), dy)))[0]
+    want, lim = mlp_reference(tail.detach(), w12, b12, w3, b3, "silu", dy)
+    for got, i in ((ys, 0), (yl[-300:], 0), (gs, 1), (gl[-300:], 1)):
+        within(got.detach(), want[i], lim[i], "the last rows")
+    assert not bool(gl[:-300].any())
+
+
+@gpu
 def test_dropout_seed_tensor_that_changes_is_noticed(dev):
     x, seed = normal((64,), 31).requires_grad_(True), torch.tensor([4], device=dev)
     y = hip_block.dropout(x, 0.5, seed)
@@ -606,6 +643,8 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
     refused(L.iff_layer_norm_forward(None, 3, 1, 1, 0, 4, 4, None, None, 0, 1e-6, None, None, None), b"type 3")
     refused(L.iff_layer_norm_forward(None, 1, 1, 1, 0, 4, 4, None, None, 2, 1e-6, None, None, None), b"parameters of type 2")
     refused(L.iff_layer_norm_forward(None, 0, 1, 1, 0, 4, 0, None, None, 0, 1e-6, None, None, None), b"bad width")
+    refused(L.iff_layer_norm_forward(16, 0, 1, 1, 0, 4, 4, None, None, 0, 1e-6, 16, 20, None), b"8-byte aligned")
+    refused(L.iff_layer_norm_forward(None, 0, 1, 1, 0, 4, (1 << 24) + 1, None, None, 0, 1e-6, None, None, None), b"bad width")
     refused(L.iff_layer_norm_forward(None, 0, 1 << 20, 1 << 20, 0, 4, 4, None, None, 0, 1e-6, None, None, None), b"bad row counts")
     refused(L.iff_layer_norm_forward(None, 0, -1, 2, 0, 4, 4, None, None, 0, 1e-6, None, None, None), b"bad row counts")
     refused(L.iff_layer_norm_forward(None, 0, 1, 1, 0, 4, 4, None, None, 0, -1.0, None, None, None), b"eps")
