@@ -540,31 +540,38 @@ __global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M
         }
 }
 
-// out[i] = sum_z part[z][i] in increasing z (+ bias of the column, N columns)
+// Sums of shares, every one a call leaves in one launch (a launch of its own costs each of them 5 us of GPU time and 4 of the host's): job j
+// from workgroup first[j] on.  Elements: out[i] = sum_z part[z][i] (+ bias of the column) in increasing z.  Columns (many shares, few sums):
+// 16 columns x 64 groups of shares per workgroup, a group in increasing order, the groups joined in order.
+struct JoinJob { const float* part; void* out; const void* bias; int64_t n, N; int Z, columns; };
+struct JoinJobs { JoinJob job[6]; unsigned first[7]; int n; };
 template <class T>
-__global__ void __launch_bounds__(256) k_ffn_join(const float* __restrict__ part, int Z, int64_t n, int64_t N, const T* __restrict__ bias,
-                                                  T* __restrict__ out) {
-    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float v = part[i];
-        for (int z = 1; z < Z; ++z) v += part[z * n + i];
-        out[i] = (T)(bias ? v + (float)bias[i % N] : v);
-    }
-}
-
-// out[c] = sum_g part[g][c]: 16 columns x 64 groups of shares per workgroup, groups joined in order
-template <class T>
-__global__ void __launch_bounds__(1024) k_ffn_join_columns(const float* __restrict__ part, int64_t G, int64_t N, T* __restrict__ out) {
+__global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
     __shared__ float s[64][17];
+    int k = 0;
+    while (k + 1 < jobs.n && blockIdx.x >= jobs.first[k + 1]) ++k;
+    const JoinJob j = jobs.job[k];
+    const unsigned wg = blockIdx.x - jobs.first[k], wgs = jobs.first[k + 1] - jobs.first[k];
+    T* const out = reinterpret_cast<T*>(j.out);
+    if (!j.columns) {
+        const T* const bias = reinterpret_cast<const T*>(j.bias);
+        for (int64_t i = wg * (int64_t)1024 + threadIdx.x; i < j.n; i += (int64_t)wgs * 1024) {
+            float v = j.part[i];
+            for (int z = 1; z < j.Z; ++z) v += j.part[z * j.n + i];
+            out[i] = (T)(bias ? v + (float)bias[i % j.N] : v);
+        }
+        return;
+    }
     const int c16 = threadIdx.x & 15, grp = threadIdx.x >> 4;
-    const int64_t c = blockIdx.x * (int64_t)16 + c16;
+    const int64_t c = wg * (int64_t)16 + c16;
     float a = 0.0f;
-    if (c < N)
+    if (c < j.n)
 #pragma unroll 8
-        for (int64_t g = grp; g < G; g += 64) a += part[g * N + c];
+        for (int g = grp; g < j.Z; g += 64) a += j.part[g * j.n + c];
     s[grp][c16] = a;
     __syncthreads();
-    if (grp == 0 && c < N) {
-        for (int j = 1; j < 64; ++j) a += s[j][c16];
+    if (grp == 0 && c < j.n) {
+        for (int i = 1; i < 64; ++i) a += s[i][c16];
         out[c] = (T)a;
     }
 }
@@ -702,22 +709,40 @@ hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
     default: return tiles<T, AK, BK, EPI, 2, 2, 1, 1, 64, 4>(g, splits, s);
     }
 }
+// the sums of shares that a call's launches leave, taken by one launch at its end
 template <class T>
-hipError_t join_shares(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out, hipStream_t s) {
-    const int64_t n = rows * N;
-    k_ffn_join<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 4096), 256, 0, s>>>(part, z, n, N, (const T*)bias, (T*)out);
-    return hipGetLastError();
-}
+struct Joins {
+    Work& w;
+    JoinJobs jobs{};
+    explicit Joins(Work& work) : w(work) {}
+    void add(JoinJob j, int64_t wgs) {
+        if (!j.n) return;
+        jobs.job[jobs.n] = j;
+        jobs.first[jobs.n + 1] = jobs.first[jobs.n] + (unsigned)wgs;
+        ++jobs.n;
+    }
+    void elements(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out) {
+        const int64_t n = rows * N;
+        add({part, out, bias, n, N, z, 0}, std::min<int64_t>((n + 1023) / 1024, 1024));
+    }
+    void columns(const float* part, int64_t shares, int64_t N, void* out) { add({part, out, nullptr, N, N, (int)shares, 1}, (N + 15) / 16); }
+    hipError_t go() {
+        if (!jobs.n || w.counting()) return hipSuccess;
+        k_ffn_join<T><<<jobs.first[jobs.n], 1024, 0, w.s>>>(jobs);
+        return hipGetLastError();
+    }
+};
 // rows `from` .. M - 1 of a product, over `splits` shares of k
 template <class T, int AK, int BK, int EPI>
-hipError_t rows_of(Work& w, Prod g, int64_t from, int shape, int splits) {
+hipError_t rows_of(Work& w, Joins<T>& joins, Prod g, int64_t from, int shape, int splits) {
     float* part = splits > 1 ? (float*)w.take((size_t)splits * (g.M - from) * g.N * 4) : nullptr;
     if (w.counting() || from == g.M) return hipSuccess;
     g.m_base = from;
     if (!part) return launch_shape<T, AK, BK, EPI>(shape, g, 1, w.s);
     g.part = part; g.rows_out = g.M - from; g.vec_out = g.N % 4 == 0;
     FFN_TRY((launch_shape<T, AK, BK, EPI>(shape, g, splits, w.s)));
-    return join_shares<T>(part, splits, g.M - from, g.N, g.bias, (T*)g.out + from * g.N, w.s);
+    joins.elements(part, splits, g.M - from, g.N, g.bias, (T*)g.out + from * g.N);
+    return hipSuccess;
 }
 template <class T, int EPI>
 Plan product_plan(const Prod& g) {
@@ -731,32 +756,28 @@ Plan product_plan(const Prod& g) {
 }
 // a product over the rows of a batch
 template <class T, int AK, int BK, int EPI>
-hipError_t product(Work& w, Prod g) {
+hipError_t product(Work& w, Joins<T>& joins, Prod g) {
     const Plan p = product_plan<T, EPI>(g);
     const int64_t M = g.M;
     g.M = p.main_rows;
-    FFN_TRY((rows_of<T, AK, BK, EPI>(w, g, 0, p.shape, p.splits)));
+    FFN_TRY((rows_of<T, AK, BK, EPI>(w, joins, g, 0, p.shape, p.splits)));
     g.M = M;
-    return rows_of<T, AK, BK, EPI>(w, g, p.main_rows, p.rest_shape, p.rest_splits);
+    return rows_of<T, AK, BK, EPI>(w, joins, g, p.main_rows, p.rest_shape, p.rest_splits);
 }
 template <class T>
-hipError_t weight_gradient(Work& w, Prod g, int64_t rows_out) {
+hipError_t weight_gradient(Work& w, Joins<T>& joins, Prod g, int64_t rows_out) {
     const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 256)), false);
     g.rows_out = rows_out;
     if (p.splits > 1) g.part = (float*)w.take((size_t)p.splits * rows_out * g.N * 4);
     if (w.counting()) return hipSuccess;
     g.vec_out = g.N % 4 == 0 && (p.splits > 1 || aligned16(g.out));
     FFN_TRY((launch_shape<T, KS, KS, EPI_OUT>(p.shape, g, p.splits, w.s)));
-    return p.splits > 1 ? join_shares<T>(g.part, p.splits, rows_out, g.N, nullptr, g.out, w.s) : hipSuccess;
-}
-template <class T>
-hipError_t join_columns(const float* part, int64_t G, int64_t N, void* out, hipStream_t s) {
-    k_ffn_join_columns<T><<<(unsigned)((N + 15) / 16), 1024, 0, s>>>(part, G, N, (T*)out);
-    return hipGetLastError();
+    if (p.splits > 1) joins.elements(g.part, p.splits, rows_out, g.N, nullptr, g.out);
+    return hipSuccess;
 }
 // shares: enough workgroups for the chip, each at least 64 rows
 template <class T>
-hipError_t colsum(Work& w, const void* a, int64_t M, int64_t N, void* out) {
+hipError_t colsum(Work& w, Joins<T>& joins, const void* a, int64_t M, int64_t N, void* out) {
     constexpr int V = 16 / (int)sizeof(T);
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>((M + 63) / 64, 128));
     float* part = (float*)w.take((size_t)shares * N * 4);
@@ -765,7 +786,8 @@ hipError_t colsum(Work& w, const void* a, int64_t M, int64_t N, void* out) {
         k_ffn_colsum<T, V><<<dim3((unsigned)((N + 32 * V - 1) / (32 * V)), (unsigned)shares), 256, 0, w.s>>>((const T*)a, M, N, part);
     else
         k_ffn_colsum<T, 1><<<dim3((unsigned)((N + 31) / 32), (unsigned)shares), 256, 0, w.s>>>((const T*)a, M, N, part);
-    return join_columns<T>(part, shares, N, out, w.s);
+    joins.columns(part, shares, N, out);
+    return hipGetLastError();
 }
 
 // what the forward pass keeps: h planes, then p and q
@@ -796,6 +818,7 @@ hipError_t forward(const FfnArgs& f, Work& w) {
         }
     }
     Packer<T> pack(w);
+    Joins<T> joins(w);
     const Operand x = pack.add(f.x, 1, f.M, f.D), w12 = pack.add(f.w12, 2, f.H, f.D), w3 = pack.add(f.w3, 1, f.O, f.H);
     FFN_TRY(pack.go());
     char* h = (char*)f.kept;
@@ -803,11 +826,12 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     Prod g{};
     g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.plane_o = f.M * HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
-    FFN_TRY((product<T, KC, KC, EPI_GATE>(w, g)));
+    FFN_TRY((product<T, KC, KC, EPI_GATE>(w, joins, g)));
     Prod d{};
     d.a = {h, HP, f.M * HP}; d.b = w3; d.ra = f.M; d.rb = f.O; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
     d.vec_out = f.O % 4 == 0 && aligned16(f.y);
-    return product<T, KC, KC, EPI_OUT>(w, d);
+    FFN_TRY((product<T, KC, KC, EPI_OUT>(w, joins, d)));
+    return joins.go();
 }
 
 template <class T>
@@ -817,6 +841,7 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     char* h = (char*)f.kept;
     const float* p = (const float*)(h + (all ? 0 : kept_h<T>(f.M, f.H)));
     Packer<T> pack(w);
+    Joins<T> joins(w);
     Operand dy{}, w3{}, w12{}, x{};
     if (hidden || f.dw3) dy = pack.add(f.dy, 1, f.M, f.O);
     if (hidden) w3 = pack.add(f.w3, 1, f.O, f.H);
@@ -831,26 +856,26 @@ hipError_t backward(const FfnArgs& f, Work& w) {
         const int slice = product_plan<T, EPI_DH>(g).shape == SHAPE_64 ? 32 : 64;
         const int64_t slices = (f.M + slice - 1) / slice;
         if (all || f.db12) g.sums = (float*)w.take((size_t)slices * 2 * f.H * 4);
-        FFN_TRY((product<T, KC, KS, EPI_DH>(w, g)));
-        if (!all && f.db12) FFN_TRY(join_columns<T>(g.sums, slices, 2 * (int64_t)f.H, f.db12, w.s));
+        FFN_TRY((product<T, KC, KS, EPI_DH>(w, joins, g)));
+        if (!all && f.db12) joins.columns(g.sums, slices, 2 * (int64_t)f.H, f.db12);
     }
     if (all || f.dx) {
         Prod g{};
         g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
-        FFN_TRY((product<T, KC, KS, EPI_OUT>(w, g)));
+        FFN_TRY((product<T, KC, KS, EPI_OUT>(w, joins, g)));
     }
     if (all || f.dw12) {
         Prod g{};
         g.a = dgu; g.b = x; g.M = 2 * HP; g.N = f.D; g.K = f.M; g.out = f.dw12; g.half_pad = HP; g.half = f.H;
-        FFN_TRY(weight_gradient<T>(w, g, 2 * (int64_t)f.H));
+        FFN_TRY(weight_gradient<T>(w, joins, g, 2 * (int64_t)f.H));
     }
     if (all || f.dw3) {
         Prod g{};
         g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
-        FFN_TRY(weight_gradient<T>(w, g, f.O));
+        FFN_TRY(weight_gradient<T>(w, joins, g, f.O));
     }
-    if (all || f.db3) FFN_TRY(colsum<T>(w, f.dy, f.M, f.O, f.db3));
-    return hipSuccess;
+    if (all || f.db3) FFN_TRY(colsum<T>(w, joins, f.dy, f.M, f.O, f.db3));
+    return joins.go();
 }
 
 template <class F>

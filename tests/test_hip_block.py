@@ -415,6 +415,9 @@ def test_offsets_past_32_bits(dev):
     x.copy_(normal((2, 64), 60, torch.float16))
     assert torch.equal(hip_block.layer_norm(x), hip_block.layer_norm(x.contiguous()))
     del base, x
+    rows = normal((2 ** 24 + 7, 1), 64, torch.float16).expand(-1, 8) * torch.arange(8, device=dev, dtype=torch.float16)
+    assert torch.equal(hip_block.layer_norm(rows)[-9:], hip_block.layer_norm(rows[-9:]))       # more rows than one launch has workgroups for
+    del rows
     M, D, H = 2 ** 20 + 300, 2048, 8
     x = torch.zeros(M, D, dtype=torch.bfloat16, device=dev)
     tail = normal((300, D), 61, torch.bfloat16)
