@@ -2,6 +2,7 @@
 
 Layout
   csrc/ + libiffnerf_hip.so   hand-written HIP kernels for gfx950 behind the C ABI of include/iffnerf_hip.h
+  hip_block.py                layer norm, gated feed-forward and dropout with their gradients (backbone training)
   _lib.py, hip_field.py, hip_identify.py   ctypes binding and handle owners (PyTorch-ROCm supplies memory/streams)
   models/, pose_estimation/, renderer.py   host-side mirror of the reference's module paths and call signatures
   synthetic.py                seeded synthetic checkpoints (no pretrained weights are available offline)
