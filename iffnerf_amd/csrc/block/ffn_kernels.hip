@@ -163,17 +163,19 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
     tn = t / rows;
 }
 
-// Tiles of 32 MR WM x 32 NR WN, 32 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
-// 1 KB per instruction, lane-linear in LDS) into a ring of NBUF buffers.  A KC tile is rows of 32 k
-// (64 B), its 16-byte chunk c in slot c ^ (row / 4 & 3); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 and 192
-// columns, whose rows are not whole 256-byte bank rows: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the lanes' SOURCE addresses and
-// keep every LDS read free of bank conflicts.
-template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
+// Tiles of 32 MR WM x 32 NR WN, 64 deep, WM x WN waves of 32 MR x 32 NR.  Operand tiles go from memory to LDS by DMA (16 bytes per lane,
+// 1 KB per instruction, lane-linear in LDS) into a ring of NBUF buffers.  A KC tile is rows of 64 k (128 B), its 16-byte chunk c in
+// slot c ^ (row / 2 & 7); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 and 192 columns, whose rows are not whole
+// 256-byte bank rows: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the
+// lanes' SOURCE addresses and keep the LDS reads free of bank conflicts.  What bounds it: the fill of LDS from L2 (a build that does
+// nothing else needs 0.6 - 0.8 of a launch) beside the matrix pipe (0.47 of F2's clocks at 16448 x 1536 x 4096, 242 us).  32-deep rings of
+// three to five buffers measured the same or slower, four waves of 128 x 128 17 % slower.
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int NBUF>
 __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
     typedef typename Mat<T>::e E;
     typedef typename Vec8<E>::t E8;
     constexpr int P = Mat<T>::P, NW = WM * WN, BM = 32 * MR * WM, BN = 32 * NR * WN;
-    constexpr int ROW = KT * 2, PA = BM * ROW / 1024 / NW, PB = BN * ROW / 1024 / NW;      // 1-KB pieces per wave and step
+    constexpr int KT = 64, ROW = KT * 2, PA = BM * ROW / 1024 / NW, PB = BN * ROW / 1024 / NW;      // 1-KB pieces per wave and step
     constexpr int TILE = (BM + BN) * ROW, GW = 16 * NR;
     constexpr int OLD = 32 * NR + 4;                                  // floats per row of a wave's output tile in LDS: conflict-free 16-byte writes down a column
     constexpr int POOL = NBUF * TILE > NW * 32 * OLD * 4 ? NBUF * TILE : NW * 32 * OLD * 4;
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
     const E* const A = reinterpret_cast<const E*>(g.a.p);
     const E* const B = reinterpret_cast<const E*>(g.b.p);
 
-    const auto swizzle = [](int r) { return KT == 64 ? (r >> 1) & 7 : (r >> 2) & 3; };
+    const auto swizzle = [](int r) { return (r >> 1) & 7; };
     const auto turn = [](int r, int width) { return width % 128 ? (r & 2) << 1 : (r & 3) << 2; };
 
     // the lane's source of each piece, in bytes from the tile's corner at the step's k (ld < 2^22: 256 rows stay below 2^31), and its first k
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
 // At most 8 rows and no gradients (serving token by token): the weights are read once and that is all the time there is, so the products are
 // vector dot products -- a wave per RW rows of the weight matrix, its lanes over k, 16 bytes per load, fp32 sums joined across the lanes --
 // and not tiles of which 8 of 128 rows would be used.  GATE: RW / 2 hidden units, their gate and their up row; else RW outputs.  The hidden
-// activation stays fp32 between the two launches.  One token, 1536 x 4096 bf16: 5.9 + 4.2 us, 3.7 TB/s of weights.
+// activation stays fp32 between the two launches.  One token, 1536 x 4096 bf16: 7 + 4 us, 3.4 TB/s of weights.
 template <class T, int V, int MM, int RW, bool GATE, class TX, class TO>
 __global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M, int64_t K, const T* __restrict__ w, int64_t N, const T* __restrict__ bias,
                                                  int act, TO* __restrict__ out) {
@@ -543,7 +545,8 @@ __global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M
 // Sums of shares, every one a call leaves in one launch (a launch of its own costs each of them 5 us of GPU time and 4 of the host's): job j
 // from workgroup first[j] on.  Elements: out[i] = sum_z part[z][i] (+ bias of the column) in increasing z.  Columns (many shares, few sums):
 // 16 columns x 64 groups of shares per workgroup, a group in increasing order, the groups joined in order.
-struct JoinJob { const float* part; void* out; const void* bias; int64_t n, N; int Z, columns; };
+enum { JOIN_ELEMENTS = 0, JOIN_COLUMNS = 1, JOIN_ELEMENTS4 = 2 };      // (the last: four at a time, where N and out allow it)
+struct JoinJob { const float* part; void* out; const void* bias; int64_t n, N; int Z, kind; };
 struct JoinJobs { JoinJob job[6]; unsigned first[7]; int n; };
 template <class T>
 __global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
@@ -553,7 +556,25 @@ __global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
     const JoinJob j = jobs.job[k];
     const unsigned wg = blockIdx.x - jobs.first[k], wgs = jobs.first[k + 1] - jobs.first[k];
     T* const out = reinterpret_cast<T*>(j.out);
-    if (!j.columns) {
+    if (j.kind == JOIN_ELEMENTS4) {
+        const T* const bias = reinterpret_cast<const T*>(j.bias);
+        for (int64_t i = (wg * (int64_t)1024 + threadIdx.x) * 4; i < j.n; i += (int64_t)wgs * 4096) {
+            float v[4], t[4];
+            Pack<float, 4>::load(j.part + i, v);
+#pragma unroll 4
+            for (int z = 1; z < j.Z; ++z) {
+                Pack<float, 4>::load(j.part + z * j.n + i, t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += t[e];
+            }
+            if (bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += (float)bias[i % j.N + e];
+            store4<T>(out + i, v);
+        }
+        return;
+    }
+    if (j.kind == JOIN_ELEMENTS) {
         const T* const bias = reinterpret_cast<const T*>(j.bias);
         for (int64_t i = wg * (int64_t)1024 + threadIdx.x; i < j.n; i += (int64_t)wgs * 1024) {
             float v = j.part[i];
@@ -643,14 +664,14 @@ struct Packer {
     }
 };
 
-template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int KT, int NBUF>
+template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int NBUF>
 hipError_t tiles(Prod g, int splits, hipStream_t s) {
     constexpr int BM = 32 * MR * WM, NT = EPI == EPI_GATE ? 16 * NR * WN : 32 * NR * WN;
     const int64_t N = EPI == EPI_OUT ? g.N : g.HP, gm = (g.M - g.m_base + BM - 1) / BM, gn = (N + NT - 1) / NT;
     if (gm <= 0 || !gn) return hipSuccess;
     if (gm * gn >= (1ll << 32) / (64 * WM * WN)) return hipErrorInvalidConfiguration;      // (a launch has fewer than 2^32 threads)
     g.k_per_split = splits > 1 ? ((g.K + splits - 1) / splits + 63) / 64 * 64 : std::max<int64_t>(g.K, 64);
-    k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, KT, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
+    k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
     return hipGetLastError();
 }
 // ---- which tiles, and how many shares of the k loop.  A round is one tile on every CU (two of the 128 x 128 ones); its time is modelled as
@@ -662,51 +683,59 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
 // A product with few tiles is bound by the latency of its steps instead: 0.85 us per 64 k of a 128 x 128 tile alone on its CU with two buffers,
 // less with four (then the tile has the CU to itself), and 64 x 64 tiles bring four times the workgroups.
 enum { SHAPE_256 = 0, SHAPE_192, SHAPE_128, SHAPE_128_DEEP, SHAPE_64, SHAPES };
-constexpr struct Shape { int bm, bn, slots; double step; } kShape[SHAPES] = {          // step: us per 64 k of a round
-    {256, 256, 256, 1.8}, {256, 192, 256, 1.42}, {128, 128, 512, 1.08}, {128, 128, 256, 0.60}, {64, 64, 512, 0.45}};
+constexpr struct Shape { int bm, bn, slots_log2; double step; } kShape[SHAPES] = {     // step: us per 64 k of a round
+    {256, 256, 8, 1.8}, {256, 192, 8, 1.42}, {128, 128, 9, 1.08}, {128, 128, 8, 0.60}, {64, 64, 9, 0.45}};
 struct Plan { int shape, splits; int64_t main_rows; int rest_shape, rest_splits; };      // the rows behind main_rows go to a launch of their own
 
-inline double round_time(int shape, int64_t M, int64_t N, int64_t K, int splits, double out_bytes) {
-    const Shape& s = kShape[shape];
-    const int64_t t = (M + s.bm - 1) / s.bm * ((N + s.bn - 1) / s.bn) * splits;
-    const double steps = (double)((K + 64 * splits - 1) / (64 * splits));
-    return (double)((t + s.slots - 1) / s.slots) * (steps * s.step + 3.0) + (double)M * N * out_bytes / 4.5e6;
-}
-inline double share_time(int64_t M, int64_t N, int splits) { return splits > 1 ? 5.0 + (double)M * N * 4 * (splits + 1) / 4.5e6 : 0.0; }
+// rows x N of C in one launch of `shape`, us (this runs at every call: nothing but the tile counts is divided per shape)
+struct Cost {
+    int64_t tiles[SHAPES]; double elements, traffic;
+    Cost(int64_t rows, int64_t N, double out_bytes) : elements((double)rows * N), traffic((double)rows * N * out_bytes / 4.5e6) {
+        for (int i = 0; i < SHAPES; ++i) tiles[i] = (rows + kShape[i].bm - 1) / kShape[i].bm * ((N + kShape[i].bn - 1) / kShape[i].bn);
+    }
+    double of(int shape, int splits, double steps) const {
+        const Shape& s = kShape[shape];
+        const int64_t rounds = (tiles[shape] * splits + (1 << s.slots_log2) - 1) >> s.slots_log2;
+        return (double)rounds * (steps * s.step + 3.0) + traffic + (splits > 1 ? 5.0 + elements * 4 * (splits + 1) / 4.5e6 : 0.0);
+    }
+};
 // out_bytes: what the epilogue moves per element of C; most: shares of the k loop that may be taken, each at least 256 deep
 inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most, bool may_rest = true) {
     Plan best{SHAPE_128, 1, M, SHAPE_128, 1};
     double least = 1e300, rest = 1e300;
-    const int64_t whole = may_rest ? M / 256 * 256 : 0;
+    const int64_t whole = may_rest && M % 256 ? M / 256 * 256 : 0;
+    const Cost all(M, N, out_bytes), behind(M - whole, N, out_bytes), front(whole, N, out_bytes);
+    const double steps_1 = (double)((K + 63) / 64);
     int rest_shape = SHAPE_128, rest_splits = 1;
-    for (int z = 1; z <= most && (z == 1 || K / z >= 256); z += z < 8 ? 1 : z < 16 ? 2 : 8)      // (1 .. 8, 10 .. 16, 24 .. 64: this runs at every call)
+    for (int z = 1; z <= most && (z == 1 || K >= 256 * (int64_t)z); z += z < 8 ? 1 : z < 16 ? 2 : 8) {      // 1 .. 8, 10 .. 16, 24 .. 64
+        const double steps = z == 1 ? steps_1 : (double)((K + 64 * z - 1) / (64 * z));
         for (int shape = SHAPE_256; shape < SHAPES; ++shape) {
             if (shape == SHAPE_192 && !may_192) continue;
-            const double all = round_time(shape, M, N, K, z, out_bytes) + share_time(M, N, z);
-            if (all < least) { least = all; best = {shape, z, M, SHAPE_128, 1}; }
-            if (!whole || whole == M || shape < SHAPE_128 || z > 16) continue;
-            const double t = 6.0 + round_time(shape, M - whole, N, K, z, out_bytes) + share_time(M - whole, N, z);
-            if (t < rest) { rest = t; rest_shape = shape; rest_splits = z; }
+            const double t = all.of(shape, z, steps);
+            if (t < least) { least = t; best = {shape, z, M, SHAPE_128, 1}; }
+            if (!whole || shape < SHAPE_128 || z > 16) continue;
+            const double r = 6.0 + behind.of(shape, z, steps);
+            if (r < rest) { rest = r; rest_shape = shape; rest_splits = z; }
         }
-    if (whole && whole < M)
-        for (int shape = SHAPE_256; shape <= SHAPE_192; ++shape) {
-            if (shape == SHAPE_192 && !may_192) continue;
-            const double two = round_time(shape, whole, N, K, 1, out_bytes) + rest;
-            if (two < least) { least = two; best = {shape, 1, whole, rest_shape, rest_splits}; }
-        }
+    }
+    for (int shape = SHAPE_256; whole && shape <= SHAPE_192; ++shape) {
+        if (shape == SHAPE_192 && !may_192) continue;
+        const double two = front.of(shape, 1, steps_1) + rest;
+        if (two < least) { least = two; best = {shape, 1, whole, rest_shape, rest_splits}; }
+    }
     return best;
 }
 
 template <class T, int AK, int BK, int EPI>
 hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
     switch (shape) {
-    case SHAPE_256: return tiles<T, AK, BK, EPI, 4, 2, 2, 4, 64, 2>(g, splits, s);
+    case SHAPE_256: return tiles<T, AK, BK, EPI, 4, 2, 2, 4, 2>(g, splits, s);
     case SHAPE_192:
-        if constexpr (AK == KS) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 64, 2>(g, splits, s);
+        if constexpr (AK == KS) return tiles<T, AK, BK, EPI, 4, 2, 2, 3, 2>(g, splits, s);
         else return hipErrorInvalidConfiguration;
-    case SHAPE_128: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 2>(g, splits, s);
-    case SHAPE_128_DEEP: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 64, 4>(g, splits, s);
-    default: return tiles<T, AK, BK, EPI, 2, 2, 1, 1, 64, 4>(g, splits, s);
+    case SHAPE_128: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 2>(g, splits, s);
+    case SHAPE_128_DEEP: return tiles<T, AK, BK, EPI, 2, 2, 2, 2, 4>(g, splits, s);
+    default: return tiles<T, AK, BK, EPI, 2, 2, 1, 1, 4>(g, splits, s);
     }
 }
 // the sums of shares that a call's launches leave, taken by one launch at its end
@@ -723,9 +752,11 @@ struct Joins {
     }
     void elements(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out) {
         const int64_t n = rows * N;
-        add({part, out, bias, n, N, z, 0}, std::min<int64_t>((n + 1023) / 1024, 1024));
+        const bool four = N % 4 == 0 && aligned16(out);
+        const int64_t per = four ? 4096 : 1024;
+        add({part, out, bias, n, N, z, four ? JOIN_ELEMENTS4 : JOIN_ELEMENTS}, std::min<int64_t>((n + per - 1) / per, 2048));
     }
-    void columns(const float* part, int64_t shares, int64_t N, void* out) { add({part, out, nullptr, N, N, (int)shares, 1}, (N + 15) / 16); }
+    void columns(const float* part, int64_t shares, int64_t N, void* out) { add({part, out, nullptr, N, N, (int)shares, JOIN_COLUMNS}, (N + 15) / 16); }
     hipError_t go() {
         if (!jobs.n || w.counting()) return hipSuccess;
         k_ffn_join<T><<<jobs.first[jobs.n], 1024, 0, w.s>>>(jobs);
