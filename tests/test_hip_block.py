@@ -531,6 +531,41 @@ def test_the_half_block_in_a_graph_and_on_other_streams(dev):
 
 
 @gpu
+def test_the_half_block_twice_from_one_graph_and_from_two_threads(dev):
+    """Gradients taken twice from a graph that is kept, and two threads that run the block at once on streams of their own: the same bits."""
+    import threading
+    args, dy = block_inputs(torch.bfloat16)
+
+    def leaves():
+        return [t.detach().clone().requires_grad_(True) for t in args]
+
+    mine = leaves()
+    y = half_block(*mine, 11)
+    first = torch.autograd.grad(y, mine, dy, retain_graph=True)
+    second = torch.autograd.grad(y, mine, dy)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    torch.cuda.synchronize()
+    got = {}
+
+    def run(k):
+        stream = torch.cuda.Stream(dev)
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                own = leaves()
+                out = half_block(*own, 11)
+                got[k] = (out.detach(), *torch.autograd.grad(out, own, dy))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert all(torch.equal(a, b) for a, b in zip((y.detach(), *first), got[k]))
+
+
+@gpu
 def test_first_derivatives_only(dev):
     x = normal((4, 16), 40).requires_grad_(True)
     g, = torch.autograd.grad(hip_block.layer_norm(x).sum(), (x,), create_graph=True)
