@@ -259,6 +259,8 @@ class _NativeLayerNorm(_NativeForward):
 class _NativeGatedMlp(_NativeForward):
     def __call__(self, x):
         m = self.module
+        if not (_just_linear(m.w12) and _just_linear(m.w3)):      # a hook or a forward of their own, installed since: theirs to run
+            return type(m).forward(m, x)
         return hip_block.gated_mlp(*_autocast(x, m.w12.weight, m.w12.bias, m.w3.weight, m.w3.bias))
 
 
@@ -282,16 +284,38 @@ class _NativeDropAdd(_NativeForward):
         return hip_block.dropout(branch.to(residual.dtype), m.p, _fresh_seed(branch), residual=residual)
 
 
+def _runs(m, cls) -> bool:
+    """m computes what ``cls`` computes: that class or a subclass without a forward of its own, and none installed on the instance."""
+    return isinstance(m, cls) and type(m).forward is cls.forward and isinstance(m.__dict__.get("forward"), (type(None), _NativeForward))
+
+
+def _just_linear(m) -> bool:
+    """m is its weight and bias and nothing else: no hook would see, or change (weight norm), what a call that skips it computes."""
+    return _runs(m, torch.nn.Linear) and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def _is_gated_silu(m: torch.nn.Module) -> bool:
+    """``w12`` and ``w3`` of matching widths, and nothing in the module that says more happens between them than SiLU."""
+    w12, w3 = getattr(m, "w12", None), getattr(m, "w3", None)
+    if not (_just_linear(w12) and _just_linear(w3) and w12.out_features == 2 * w3.in_features):
+        return False
+    if not isinstance(m.__dict__.get("forward"), (type(None), _NativeForward)):
+        return False
+    more = [c for name, c in m.named_children() if name not in ("w12", "w3")]
+    more += [m.__dict__[name] for name in ("act", "act_fn", "activation") if name in m.__dict__]
+    return all(c is None or c is F.silu or c == "silu" or isinstance(c, (torch.nn.SiLU, torch.nn.Identity))
+               or (isinstance(c, torch.nn.Dropout) and c.p == 0.0) for c in more)
+
+
 def _native_forward(m: torch.nn.Module):
     from .pose_estimation.backbone import _DropAdd
-    if isinstance(m, torch.nn.LayerNorm) and len(m.normalized_shape) == 1:
+    if _runs(m, torch.nn.LayerNorm) and len(m.normalized_shape) == 1:
         return _NativeLayerNorm(m)
-    if isinstance(m, torch.nn.Dropout) and not m.inplace:
+    if _runs(m, torch.nn.Dropout) and not m.inplace:
         return _NativeDropout(m)
-    if isinstance(m, _DropAdd):
+    if _runs(m, _DropAdd):
         return _NativeDropAdd(m)
-    w12, w3 = getattr(m, "w12", None), getattr(m, "w3", None)
-    if isinstance(w12, torch.nn.Linear) and isinstance(w3, torch.nn.Linear) and w12.out_features == 2 * w3.in_features:
+    if _is_gated_silu(m):
         return _NativeGatedMlp(m)
     return None
 
@@ -301,7 +325,8 @@ def train_natively(module: torch.nn.Module) -> torch.nn.Module:
     pose_estimation/train.py:97-119 back-propagates through -- on ``hip_block``'s operators, forward and backward, and return THE SAME
     module.  As with ``serve_natively`` nothing is wrapped: classes, parameters and ``state_dict`` keys stay, one instance attribute
     ``forward`` per sub-module is installed.  The module then needs GPU tensors; values differ from stock torch by rounding, and a dropout's
-    mask comes from another generator (seeded by torch's).  ``train_stock(module)`` removes it; without this call nothing changes."""
+    mask comes from another generator (seeded by torch's).  A sub-module with a forward of its own, or a gated feed-forward that holds more than
+``w12``, ``w3`` and SiLU, is left as it is.  ``train_stock(module)`` removes it; without this call nothing changes."""
     for m in module.modules():
         f = _native_forward(m)
         if f is not None:

@@ -603,6 +603,55 @@ def test_train_natively_keeps_the_module():
             backbone(**bad)
 
 
+def test_train_natively_leaves_what_computes_something_else():
+    """Subclasses and instances with a forward of their own, gated feed-forwards with another activation or more inside, projections that a
+    hook watches or changes (weight norm): each keeps its own forward and its own result, on the CPU here."""
+    from iffnerf_amd import hip_vit
+    nn = torch.nn
+
+    class ChannelNorm(nn.LayerNorm):
+        def forward(self, x):
+            return super().forward(x.movedim(1, -1)).movedim(-1, 1)
+
+    class Scaled(nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Gated(nn.Module):
+        def __init__(self, linear=nn.Linear, **more):
+            super().__init__()
+            self.w12, self.w3 = linear(8, 12), nn.Linear(6, 8)
+            for name, value in more.items():
+                setattr(self, name, value)
+
+        def forward(self, x):
+            g, u = self.w12(x).chunk(2, dim=-1)
+            return self.w3(getattr(self, "act", nn.functional.silu)(g) * u)
+
+    patched = nn.LayerNorm(8)
+    patched.forward = lambda x: x + 1
+    others = [ChannelNorm(8), patched, Gated(Scaled), Gated(act=nn.GELU()), Gated(act=nn.functional.gelu), Gated(inner=nn.LayerNorm(6)),
+              Gated(drop=nn.Dropout(0.1))]
+    watched = Gated()
+    seen = []
+    watched.w12.register_forward_hook(lambda *a: seen.append(1))
+    whole = nn.ModuleList([*others, watched]).eval()
+    x = torch.randn(2, 8, generator=torch.Generator().manual_seed(1))
+    want = [m(x) for m in whole if not hasattr(m, "inner")]
+    hip_vit.train_natively(whole)
+    assert not any("forward" in m.__dict__ for m in whole if m is not patched)
+    assert all(torch.equal(m(x), w) for m, w in zip((m for m in whole if not hasattr(m, "inner")), want)) and len(seen) == 2
+    for m in (Gated(), Gated(act=nn.SiLU()), Gated(drop=nn.Dropout(0.0))):
+        hip_vit.train_natively(m)
+        assert "forward" in m.__dict__
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            m(x)
+        m.w3.register_forward_pre_hook(lambda *a: None)              # (installed later: from then on the module's own forward)
+        assert torch.equal(m(x), type(m).forward(m, x))
+    hip_vit.train_stock(patched)
+    assert torch.equal(patched(x), x + 1)
+
+
 @gpu
 @pytest.mark.parametrize("ffn", ["mlp", "swiglu"])
 def test_a_backbone_trains_on_them(dev, ffn, monkeypatch):
