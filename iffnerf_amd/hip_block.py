@@ -20,16 +20,17 @@ from . import _lib
 from ._lib import check
 
 
-# A small call is bound by the host: what a backward pass runs on autograd's own thread costs three times what it costs in a loop
-# (forward + backward of a 8 x 64 dropout: 108 us with the guards of the other wrappers, 60-70 us with these, 55 us for torch's own product).
+# A small call is bound by the host: what a backward pass runs on autograd's own thread costs three times what it costs in a loop (torch's
+# current_device there 2.5 us, the binding under it 0.3), so the backward passes look nothing up that the forward pass knew
+# (forward + backward of 8 x 64 values: dropout 66 us, 72 with those lookups; norm with parameters 96, 106; torch's own product 41).
 _TYPES = _lib.TYPES
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _run(name: str, device: torch.device, *args) -> None:
-    """Entry point ``name`` with ``args`` on the current stream of ``device``."""
-    i, fn = device.index, getattr(_lib._lib or _lib.lib(), name)
-    if i == torch.cuda.current_device():
+def _run(name: str, x: torch.Tensor, *args) -> None:
+    """Entry point ``name`` with ``args`` on the current stream of x's device."""
+    i, fn = x.get_device(), getattr(_lib._lib or _lib.lib(), name)
+    if i == _current_device():
         rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(i):
@@ -75,6 +76,14 @@ def _beside(t: torch.Tensor, x: torch.Tensor, name: str, shape, *types) -> torch
     return t.contiguous()
 
 
+def _trains(*tensors: Optional[torch.Tensor]) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -108,9 +117,10 @@ def _rows(x: torch.Tensor):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _layer_norm(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.bias_type = None if bias is None else bias.dtype
+        rows = _rows(x)
+        y, stats, par = _layer_norm(x, rows, weight, bias, eps, True)
+        ctx.save_for_backward(rows[0], weight, stats)
+        ctx.how = (*rows[1:], x.shape[-1], _TYPES[x.dtype], par)
         return y
 
     @staticmethod
@@ -118,29 +128,28 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        xr, n0, n1, s0, s1 = _rows(x)
-        D, dy = x.shape[-1], dy.contiguous()
-        par = weight.dtype if weight is not None else ctx.bias_type if ctx.bias_type is not None else x.dtype
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        n0, n1, s0, s1, D, ty, par = ctx.how
+        dy = dy.contiguous()
+        dx = torch.empty_like(dy) if need_x else None
         dw = x.new_empty((D,), dtype=par) if need_w else None
         db = x.new_empty((D,), dtype=par) if need_b else None
         nbytes, ws = 0, None
         if need_w or need_b:
             nbytes = _bytes("iff_layer_norm_backward_workspace", n0 * n1, D)
             ws = _workspace(nbytes, x)
-        _run("iff_layer_norm_backward", x.device, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, D, _ptr(weight), _TYPES[par],
-             stats.data_ptr(), dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+        _run("iff_layer_norm_backward", x, x.data_ptr(), ty, n0, n1, s0, s1, D, _ptr(weight), _TYPES[par], stats.data_ptr(), dy.data_ptr(),
+             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, dw, db, None
 
 
-def _layer_norm(x, weight, bias, eps, keep):
-    xr, n0, n1, s0, s1 = _rows(x)
+def _layer_norm(x, rows, weight, bias, eps, keep):
+    xr, n0, n1, s0, s1 = rows
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = x.new_empty((n0 * n1, 2), dtype=torch.float32) if keep else None
     par = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    _run("iff_layer_norm_forward", x.device, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, x.shape[-1], _ptr(weight), _ptr(bias), _TYPES[par],
+    _run("iff_layer_norm_forward", x, xr.data_ptr(), _TYPES[x.dtype], n0, n1, s0, s1, x.shape[-1], _ptr(weight), _ptr(bias), _TYPES[par],
          eps, y.data_ptr(), _ptr(stats))
-    return y, stats
+    return y, stats, par
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
@@ -156,9 +165,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         weight = _beside(weight, x, "layer_norm: weight", x.shape[-1:], torch.float32, x.dtype)
     if bias is not None:
         bias = _beside(bias, x, "layer_norm: bias", x.shape[-1:], *((torch.float32, x.dtype) if weight is None else (weight.dtype,)))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _trains(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _layer_norm(x, weight, bias, float(eps), False)[0]
+    return _layer_norm(x, _rows(x), weight, bias, float(eps), False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------- gated feed-forward
@@ -167,17 +176,19 @@ def _mlp_forward(x, w12, b12, w3, b3, act, keep):
     O, H = w3.shape
     ty = _TYPES[x.dtype]
     y = x.new_empty((M, O))
-    kept = x.new_empty((_bytes("iff_gated_mlp_kept_bytes", ty, M, D, H, O),), dtype=torch.uint8) if keep else None
-    ws = _workspace(_bytes("iff_gated_mlp_forward_workspace", ty, M, D, H, O), x)
-    _run("iff_gated_mlp_forward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), _ptr(b12), w3.data_ptr(), _ptr(b3), act, y.data_ptr(),
-         _ptr(kept), kept.numel() if keep else 0, ws.data_ptr(), ws.numel())
-    return y, kept
+    kept_bytes = _bytes("iff_gated_mlp_kept_bytes", ty, M, D, H, O) if keep else 0
+    kept = x.new_empty((kept_bytes,), dtype=torch.uint8) if keep else None
+    nbytes = _bytes("iff_gated_mlp_forward_workspace", ty, M, D, H, O)
+    ws = _workspace(nbytes, x)
+    _run("iff_gated_mlp_forward", x, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), _ptr(b12), w3.data_ptr(), _ptr(b3), act, y.data_ptr(),
+         _ptr(kept), kept_bytes, ws.data_ptr(), nbytes)
+    return y, kept, (ty, M, D, H, O)
 
 
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w12, b12, w3, b3, act):
-        y, kept = _mlp_forward(x, w12, b12, w3, b3, act, True)
+        y, kept, ctx.sizes = _mlp_forward(x, w12, b12, w3, b3, act, True)
         ctx.save_for_backward(x, w12, w3, kept)
         return y
 
@@ -185,18 +196,18 @@ class _GatedMlp(torch.autograd.Function):
     @_first_derivative
     def backward(ctx, dy):
         x, w12, w3, kept = ctx.saved_tensors
-        M, D = x.shape
-        O, H = w3.shape
-        ty, dy = _TYPES[x.dtype], dy.contiguous()
-        need = ctx.needs_input_grad
+        sizes = ctx.sizes
+        ty, M, D, H, O = sizes
+        dy, need = dy.contiguous(), ctx.needs_input_grad
         dx = x.new_empty((M, D)) if need[0] else None
         dw12 = x.new_empty((2 * H, D)) if need[1] else None
         db12 = x.new_empty((2 * H,)) if need[2] else None
         dw3 = x.new_empty((O, H)) if need[3] else None
         db3 = x.new_empty((O,)) if need[4] else None
-        ws = _workspace(_bytes("iff_gated_mlp_backward_workspace", ty, M, D, H, O), x)
-        _run("iff_gated_mlp_backward", x.device, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), kept.data_ptr(),
-             dy.data_ptr(), _ptr(dx), _ptr(dw12), _ptr(db12), _ptr(dw3), _ptr(db3), ws.data_ptr(), ws.numel())
+        nbytes = _bytes("iff_gated_mlp_backward_workspace", *sizes)
+        ws = _workspace(nbytes, x)
+        _run("iff_gated_mlp_backward", x, x.data_ptr(), ty, M, D, H, O, w12.data_ptr(), w3.data_ptr(), kept.data_ptr(),
+             dy.data_ptr(), _ptr(dx), _ptr(dw12), _ptr(db12), _ptr(dw3), _ptr(db3), ws.data_ptr(), nbytes)
         return dx, dw12, db12, dw3, db3, None
 
 
@@ -219,7 +230,7 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
     b3 = None if b3 is None else _beside(b3, x, "gated_mlp: b3", (O,), x.dtype)
     x2 = x.reshape(-1, D).contiguous()
     act = _lib.ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w12, b12, w3, b3)):
+    if _trains(x2, w12, b12, w3, b3):
         y = _GatedMlp.apply(x2, w12, b12, w3, b3, act)
     else:
         y = _mlp_forward(x2, w12, b12, w3, b3, act, False)[0]
@@ -229,7 +240,7 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
 # ---------------------------------------------------------------------------------------------------- dropout
 def _dropout(x, residual, threshold, seed, seed_dev, offset):
     y = torch.empty_like(x)
-    _run("iff_dropout", x.device, x.data_ptr(), _TYPES[x.dtype], x.numel(), _ptr(residual), threshold, seed, _ptr(seed_dev), offset, y.data_ptr())
+    _run("iff_dropout", x, x.data_ptr(), _TYPES[x.dtype], x.numel(), _ptr(residual), threshold, seed, _ptr(seed_dev), offset, y.data_ptr())
     return y
 
 
@@ -270,6 +281,6 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
         residual = _beside(residual, x, "dropout: residual", x.shape, x.dtype)
     threshold = int(math.floor(p * 65536 + 0.5))
     x = x.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _trains(x, residual):
         return _Dropout.apply(x, residual, threshold, seed, seed_dev, offset)
     return _dropout(x, residual, threshold, seed, seed_dev, offset)
