@@ -75,6 +75,18 @@ __device__ __forceinline__ void store_planes(typename Mat<T>::e* o, int64_t plan
 #pragma unroll
     for (int p = 0; p < P; ++p) *reinterpret_cast<E4*>(o + p * plane) = t[p];
 }
+// what store_planes of a 16-bit type left of four values (nothing of an infinity or a NaN)
+template <class T>
+__device__ __forceinline__ void store_rest(T* o, const float v[4]) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float r = (float)(T)v[i];
+        t[i] = (T)(__builtin_isfinite(r) ? v[i] - r : 0.0f);
+    }
+    *reinterpret_cast<T4*>(o) = t;
+}
 template <class T>
 __device__ __forceinline__ void store4(T* o, const float v[4]) {
     typedef T T4 __attribute__((ext_vector_type(4)));
@@ -83,10 +95,10 @@ __device__ __forceinline__ void store4(T* o, const float v[4]) {
 
 __host__ __device__ constexpr int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// Up to four matrices in one launch, job j from workgroup first[j] on: src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind
+// Up to six matrices in one launch, job j from workgroup first[j] on: src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind
 // column C and behind row R of a half; 8 columns per thread
 struct PackJob { const void* src; void* dst; int64_t R, RP, C, CP, rows_out; int vec; };
-struct PackJobs { PackJob job[4]; unsigned first[5]; int n; };
+struct PackJobs { PackJob job[6]; unsigned first[7]; int n; };
 template <class T>
 __global__ void __launch_bounds__(256) k_ffn_pack(PackJobs jobs) {
     typedef typename Mat<T>::e E;
@@ -138,6 +150,8 @@ struct Prod {
     // EPI_DH: out = [dg | du] planes of ld ldo, du at column HP
     // and with `sums`: [M / 32 MR][2H] column sums of dg and du (fp32, before they are rounded) over a wave's rows
     int64_t up_row, HP, ldo, plane_o; float* p; float* q; int act; float* sums;
+    // EPI_GATE and EPI_DH of a 16-bit type: what rounding row m leaves, itself rounded, this many elements behind it (0: not kept)
+    int64_t rest;
 };
 
 __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0, 0};
@@ -367,7 +381,9 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
                 pv[i] = in ? uv * df : 0.0f;
                 v[i] = in ? f : 0.0f;
             }
-            store_planes<T>(reinterpret_cast<E*>(g.out) + m * g.ldo + n, g.plane_o, hv);
+            E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
+            store_planes<T>(o, g.plane_o, hv);
+            if (P == 1 && !IN && g.rest) store_rest<E>(o + g.rest, hv);          // (the rows it is kept for never fill a tile)
             if (g.p) {
                 Pack<float, 4>::store(g.p + m * g.HP + n, pv);
                 Pack<float, 4>::store(g.q + m * g.HP + n, v);
@@ -393,6 +409,7 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
             E* o = reinterpret_cast<E*>(g.out) + m * g.ldo + n;
             store_planes<T>(o, g.plane_o, p);
             store_planes<T>(o + g.HP, g.plane_o, q);
+            if (P == 1 && !IN && g.rest) { store_rest<E>(o + g.rest, p); store_rest<E>(o + g.rest + g.HP, q); }
         } else {
             int64_t row = m;
             if (!IN && g.half_pad) {
@@ -644,18 +661,19 @@ struct Packer {
     Work& w;
     PackJobs jobs{};
     explicit Packer(Work& work) : w(work) {}
-    // src [halves x R][C]; where the size is counted the copy is too (whether a start is 16-byte aligned must not change it)
-    Operand add(const void* src, int64_t halves, int64_t R, int64_t C) {
+    // src [halves x R][C]; where the size is counted the copy is too (whether a start is 16-byte aligned must not change it).  `times`: the
+    // rows that many times over (16-bit types)
+    Operand add(const void* src, int64_t halves, int64_t R, int64_t C, int times = 1) {
         const int64_t RP = halves > 1 ? pad8(R) : R, CP = pad8(C), rows = halves * RP;
-        if (Mat<T>::P == 1 && CP == C && RP == R && !w.counting() && aligned16(src)) return {src, CP, rows * CP};
-        void* dst = w.take(planes_bytes<T>(rows, CP));
-        if (!w.counting() && rows) {
+        if (Mat<T>::P == 1 && CP == C && RP == R && times == 1 && !w.counting() && aligned16(src)) return {src, CP, rows * CP};
+        char* dst = (char*)w.take(planes_bytes<T>(times * rows, CP));
+        for (int i = 0; i < times && !w.counting() && rows; ++i) {
             const int64_t n = rows * CP / 8;
-            jobs.job[jobs.n] = {src, dst, R, RP, C, CP, rows, aligned16(src) && CP == C};
+            jobs.job[jobs.n] = {src, dst + i * planes_bytes<T>(rows, CP), R, RP, C, CP, rows, aligned16(src) && CP == C};
             jobs.first[jobs.n + 1] = jobs.first[jobs.n] + (unsigned)std::min<int64_t>((n + 255) / 256, 4096);
             ++jobs.n;
         }
-        return {dst, CP, rows * CP};
+        return {dst, CP, times * rows * CP};
     }
     hipError_t go() {
         if (!jobs.n) return hipSuccess;
@@ -795,6 +813,20 @@ hipError_t product(Work& w, Joins<T>& joins, Prod g) {
     g.M = M;
     return rows_of<T, AK, BK, EPI>(w, joins, g, p.main_rows, p.rest_shape, p.rest_splits);
 }
+// a product over the rows of a batch whose A holds them twice, rounded and what the rounding left: both halves are shares of one sum
+template <class T, int BK>
+hipError_t product_of_pairs(Work& w, Joins<T>& joins, Prod g) {
+    g.ra = g.rows_out = 2 * g.M;
+    const int64_t M = g.M;
+    g.M *= 2;
+    const Plan p = product_plan<T, EPI_OUT>(g);                       // (at most 2 FEW rows: one launch)
+    g.part = (float*)w.take((size_t)p.splits * g.M * g.N * 4);
+    if (w.counting()) return hipSuccess;
+    g.vec_out = g.N % 4 == 0;
+    FFN_TRY((launch_shape<T, KC, BK, EPI_OUT>(p.shape, g, p.splits, w.s)));
+    joins.elements(g.part, 2 * p.splits, M, g.N, g.bias, g.out);
+    return hipSuccess;
+}
 template <class T>
 hipError_t weight_gradient(Work& w, Joins<T>& joins, Prod g, int64_t rows_out) {
     const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 256)), false);
@@ -821,10 +853,14 @@ hipError_t colsum(Work& w, Joins<T>& joins, const void* a, int64_t M, int64_t N,
     return hipGetLastError();
 }
 
-// what the forward pass keeps: h planes, then p and q
-template <class T> inline size_t kept_h(int64_t M, int64_t H) { return up256(planes_bytes<T>(M, pad8(H))); }
-
+// A few rows' h and [dg | du] keep what their rounding leaves next to them, as that many more rows: with so few, the error of rounding h is not
+// averaged (1 to 3 rows of fp16: up to 1.55 of the result's own rounding in y and dW3, 1.41 with many), and twice the rows fit in the same tile.
 constexpr int FEW = 8;
+template <class T> inline bool in_pairs(int64_t M) { return Mat<T>::P == 1 && M <= FEW; }
+
+// what the forward pass keeps: h planes, then p and q
+template <class T> inline size_t kept_h(int64_t M, int64_t H) { return up256(planes_bytes<T>(in_pairs<T>(M) ? 2 * M : M, pad8(H))); }
+
 template <class T, int V, int MM, int RW>
 hipError_t few_go(const FfnArgs& f, float* h, hipStream_t s) {
     const int64_t units = ((int64_t)f.H + RW / 2 - 1) / (RW / 2), outs = ((int64_t)f.O + RW / 2 - 1) / (RW / 2);
@@ -853,15 +889,17 @@ hipError_t forward(const FfnArgs& f, Work& w) {
     const Operand x = pack.add(f.x, 1, f.M, f.D), w12 = pack.add(f.w12, 2, f.H, f.D), w3 = pack.add(f.w3, 1, f.O, f.H);
     FFN_TRY(pack.go());
     char* h = (char*)f.kept;
-    if (!h) h = (char*)w.take(planes_bytes<T>(f.M, HP));
+    if (!h) h = (char*)w.take(kept_h<T>(f.M, f.H));
     Prod g{};
     g.a = x; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.D; g.out = h; g.bias = f.b12; g.act = f.act; g.HP = HP; g.ldo = HP; g.plane_o = f.M * HP; g.up_row = HP;
     if (f.kept) { g.p = (float*)(h + kept_h<T>(f.M, f.H)); g.q = g.p + f.M * HP; }
+    if (in_pairs<T>(f.M)) g.rest = f.M * HP;
     FFN_TRY((product<T, KC, KC, EPI_GATE>(w, joins, g)));
     Prod d{};
     d.a = {h, HP, f.M * HP}; d.b = w3; d.ra = f.M; d.rb = f.O; d.M = f.M; d.N = f.O; d.K = f.H; d.out = f.y; d.bias = f.b3;
     d.vec_out = f.O % 4 == 0 && aligned16(f.y);
-    FFN_TRY((product<T, KC, KC, EPI_OUT>(w, joins, d)));
+    if (in_pairs<T>(f.M)) FFN_TRY((product_of_pairs<T, KC>(w, joins, d)));
+    else FFN_TRY((product<T, KC, KC, EPI_OUT>(w, joins, d)));
     return joins.go();
 }
 
@@ -869,21 +907,22 @@ template <class T>
 hipError_t backward(const FfnArgs& f, Work& w) {
     const int64_t HP = pad8(f.H);
     const bool all = w.counting(), hidden = all || f.dx || f.dw12 || f.db12;
+    const int times = in_pairs<T>(f.M) ? 2 : 1;
     char* h = (char*)f.kept;
     const float* p = (const float*)(h + (all ? 0 : kept_h<T>(f.M, f.H)));
     Packer<T> pack(w);
     Joins<T> joins(w);
     Operand dy{}, w3{}, w12{}, x{};
-    if (hidden || f.dw3) dy = pack.add(f.dy, 1, f.M, f.O);
+    if (hidden || f.dw3) dy = pack.add(f.dy, 1, f.M, f.O, times);
     if (hidden) w3 = pack.add(f.w3, 1, f.O, f.H);
     if (all || f.dx) w12 = pack.add(f.w12, 2, f.H, f.D);
-    if (all || f.dw12) x = pack.add(f.x, 1, f.M, f.D);
+    if (all || f.dw12) x = pack.add(f.x, 1, f.M, f.D, times);
     FFN_TRY(pack.go());
-    const Operand dgu{hidden ? w.take(planes_bytes<T>(f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
+    const Operand dgu{hidden ? w.take(planes_bytes<T>(times * f.M, 2 * HP)) : nullptr, 2 * HP, f.M * 2 * HP};
     if (hidden) {
         Prod g{};
         g.a = dy; g.b = w3; g.ra = f.M; g.M = f.M; g.N = f.H; g.K = f.O; g.out = const_cast<void*>(dgu.p); g.HP = HP; g.ldo = 2 * HP; g.plane_o = dgu.plane;
-        g.p = const_cast<float*>(p); g.q = g.p + f.M * HP;
+        g.p = const_cast<float*>(p); g.q = g.p + f.M * HP; g.rest = times == 2 ? dgu.plane : 0;
         const int slice = product_plan<T, EPI_DH>(g).shape == SHAPE_64 ? 32 : 64;
         const int64_t slices = (f.M + slice - 1) / slice;
         if (all || f.db12) g.sums = (float*)w.take((size_t)slices * 2 * f.H * 4);
@@ -893,16 +932,17 @@ hipError_t backward(const FfnArgs& f, Work& w) {
     if (all || f.dx) {
         Prod g{};
         g.a = dgu; g.b = w12; g.ra = f.M; g.M = f.M; g.N = f.D; g.K = 2 * HP; g.out = f.dx; g.vec_out = f.D % 4 == 0 && aligned16(f.dx);
-        FFN_TRY((product<T, KC, KS, EPI_OUT>(w, joins, g)));
+        if (times == 2) FFN_TRY((product_of_pairs<T, KS>(w, joins, g)));
+        else FFN_TRY((product<T, KC, KS, EPI_OUT>(w, joins, g)));
     }
     if (all || f.dw12) {
         Prod g{};
-        g.a = dgu; g.b = x; g.M = 2 * HP; g.N = f.D; g.K = f.M; g.out = f.dw12; g.half_pad = HP; g.half = f.H;
+        g.a = dgu; g.b = x; g.M = 2 * HP; g.N = f.D; g.K = times * f.M; g.out = f.dw12; g.half_pad = HP; g.half = f.H;
         FFN_TRY(weight_gradient<T>(w, joins, g, 2 * (int64_t)f.H));
     }
     if (all || f.dw3) {
         Prod g{};
-        g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = f.M; g.out = f.dw3;
+        g.a = dy; g.b = {h, HP, f.M * HP}; g.M = f.O; g.N = f.H; g.K = times * f.M; g.out = f.dw3;
         FFN_TRY(weight_gradient<T>(w, joins, g, f.O));
     }
     if (all || f.db3) FFN_TRY(colsum<T>(w, joins, f.dy, f.M, f.O, f.db3));

@@ -181,17 +181,18 @@ def act64(g, name):
     return g * c, c + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
 
 
-def mlp_reference(x, w12, b12, w3, b3, act, dy):
+def mlp_reference(x, w12, b12, w3, b3, act, dy, pairs=False):
     """(y, dx, dw12, db12, dw3, db3) in 64 bits with a bound on what the operator loses before the last rounding.  A product over K runs
     as a chain of K / 16 matrix instructions (six times as many in fp32), 16 + 8 more for the adds inside one, the bias and the join of a
     split; an instruction may truncate: twice.  h and [dg | du] are rounded to the type (u) on the way; |act'| < 1.13, |act''| < 0.8; the
-    activation's own evaluation is good to (4 + |g|) 2^-23."""
-    u = U[x.dtype]
+    activation's own evaluation is good to (4 + |g|) 2^-23.  ``pairs``: what the rounding of h and [dg | du] leaves is kept, rounded (u u),
+    in products of twice as many terms."""
+    u = U[x.dtype] ** 2 if pairs else U[x.dtype]
     six = 6 if x.dtype == torch.float32 else 1
     u_way = 0.0 if x.dtype == torch.float32 else u                         # (fp32 h and [dg | du] are split exactly, but are fp32: E below)
 
     def depth(k):
-        return 2.0 * (six * k / 16.0 + 24.0) * E
+        return 2.0 * (six * (2 if pairs else 1) * k / 16.0 + 24.0) * E
 
     X, W, V, G = x.double(), w12.double(), w3.double(), dy.double()
     H = V.shape[1]
@@ -252,6 +253,24 @@ def check_mlp(x, w12, b12, w3, b3, dy, act):
     (300, 40, 520, 24, "gelu", True), (515, 256, 256, 256, "silu", False), (1100, 96, 328, 104, "gelu", True), (1031, 97, 259, 101, "silu", True)])
 def test_gated_mlp(dev, M, D, H, O, act, bias, dtype):
     check_mlp(*make_mlp(M, D, H, O, dtype, bias, seed=M + D), act)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("M,D,H,O,act,bias", [
+    (1, 1, 1, 1, "silu", True), (1, 384, 1024, 384, "gelu", True), (2, 568, 2392, 568, "gelu", False), (3, 387, 1029, 395, "silu", True),
+    (8, 1536, 4096, 1536, "silu", True), (8, 65, 67, 66, "gelu", True)])
+def test_gated_mlp_few_rows_are_exact_to_one_rounding(dev, M, D, H, O, act, bias, dtype):
+    """Up to 8 rows the hidden activation and its gradient keep what their rounding leaves: every result is its own rounding off, and no more."""
+    x, w12, b12, w3, b3, dy = make_mlp(M, D, H, O, dtype, bias, seed=7 * M + D)
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w12, b12, w3, b3)]
+    y = hip_block.gated_mlp(*leaves, activation=act)
+    live = [i for i, t in enumerate(leaves) if t is not None]
+    grads = torch.autograd.grad(y, [leaves[i] for i in live], dy)
+    want, lim = mlp_reference(x, w12, b12, w3, b3, act, dy, pairs=True)
+    within(y.detach(), want[0], lim[0], "y")
+    for i, g in zip(live, grads):
+        within(g, want[1 + i], lim[1 + i], NAMES[i])
 
 
 # sizes at which each tile shape and each way of covering the rows is taken: whole 256 x 256 tiles, 256 x 192 ones in every layout, rows left to a
