@@ -216,8 +216,8 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
     """Gated feed-forward block: ``[g | u] = x @ w12.T + b12``, ``(act(g) * u) @ w3.T + b3``.  ``x`` [..., D], ``w12`` [2 H, D] (gate rows
     first -- the ``w12`` / ``w3`` layout of DINOv2's gated feed-forward), ``w3`` [O, H], biases [2 H] / [O] or None; one type and device.
     ``activation``: "silu" or "gelu" (exact).  Differentiable in all five.  The hidden activation is rounded to the type once (up to 8
-    rows it has twice the type's precision); what the backward pass keeps next to it is fp32.  fp32 operands are multiplied as three bf16 pieces each, in fp32's accuracy; an infinite
-    fp32 operand gives NaN."""
+    rows it has twice the type's precision); what the backward pass keeps next to it is fp32.  fp32 operands are multiplied as three bf16
+    pieces each, in fp32's accuracy; an infinite fp32 operand gives NaN."""
     _serves(x, "gated_mlp: x")
     if activation not in _lib.ACTIVATIONS:
         raise RuntimeError(f"gated_mlp: activation must be one of {sorted(_lib.ACTIVATIONS)} (got {activation!r})")

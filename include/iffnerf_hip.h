@@ -569,7 +569,8 @@ int iff_layer_norm_backward(const void* x, int32_t x_type, int64_t n0, int64_t n
  *   [g | u] = x w12^T + b12,  h = act(g) u,  y = h w3^T + b3
  * x [M, D], w12 [2H, D] (gate rows first), w3 [O, H], b12_opt [2H], b3_opt [O], y [M, O]: one type, contiguous; D, 2H, O <= 2^21.
  * kept_opt (iff_gated_mlp_kept_bytes, opaque) is what the backward pass reads of the hidden activation: h rounded to the type (up to
- * 8 rows of a 16-bit type also what that leaves), and u act'(g) and act(g) in fp32.  Workspaces and kept are 16-byte aligned; a workspace is free again when the call's kernels have run. */
+ * 8 rows of a 16-bit type also what that leaves), and u act'(g) and act(g) in fp32.  Workspaces and kept are
+ * 16-byte aligned; a workspace is free again when the call's kernels have run. */
 size_t iff_gated_mlp_kept_bytes(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
 size_t iff_gated_mlp_forward_workspace(int32_t type, int64_t M, int32_t D, int32_t H, int32_t O);
 int iff_gated_mlp_forward(const void* x, int32_t type, int64_t M, int32_t D, int32_t H, int32_t O, const void* w12, const void* b12_opt,
