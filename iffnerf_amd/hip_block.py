@@ -88,6 +88,15 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _saved(t: torch.Tensor, shape, dtype: torch.dtype, device: int, name: str) -> torch.Tensor:
+    """A saved tensor as the backward pass is handed it, any strides.  A hook on saved tensors (``save_on_cpu``, compression) may have put a
+    copy in its place: its values are what was saved, its strides need not be, and another shape, type or device is not read."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+        raise RuntimeError(f"{name}: what was saved for the backward pass came back as {tuple(t.shape)} {t.dtype} on {t.device}; saved was "
+                           f"{tuple(shape)} {dtype} on GPU {device}")
+    return t
+
+
 def _workspace(nbytes: int, x: torch.Tensor) -> torch.Tensor:
     return x.new_empty((max(nbytes, 16),), dtype=torch.uint8)
 
@@ -120,7 +129,7 @@ class _LayerNorm(torch.autograd.Function):
         rows = _rows(x)
         y, stats, par = _layer_norm(x, rows, weight, bias, eps, True)
         ctx.save_for_backward(rows[0], weight, stats)
-        ctx.how = (*rows[1:], x.shape[-1], _TYPES[x.dtype], par)
+        ctx.how = (rows[0].stride(), rows[1:], x.shape[-1], _TYPES[x.dtype], par)
         return y
 
     @staticmethod
@@ -128,7 +137,14 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        n0, n1, s0, s1, D, ty, par = ctx.how
+        strides, rows, D, ty, par = ctx.how
+        dev = dy.get_device()
+        if _saved(x, dy.shape, dy.dtype, dev, "layer_norm").stride() != strides:
+            x, *rows = _rows(x)
+        n0, n1, s0, s1 = rows
+        stats = _saved(stats, (n0 * n1, 2), torch.float32, dev, "layer_norm").contiguous()
+        if weight is not None:
+            weight = _saved(weight, (D,), par, dev, "layer_norm").contiguous()
         dy = dy.contiguous()
         dx = torch.empty_like(dy) if need_x else None
         dw = x.new_empty((D,), dtype=par) if need_w else None
@@ -198,6 +214,11 @@ class _GatedMlp(torch.autograd.Function):
         x, w12, w3, kept = ctx.saved_tensors
         sizes = ctx.sizes
         ty, M, D, H, O = sizes
+        dt, dev = dy.dtype, dy.get_device()
+        x = _saved(x, (M, D), dt, dev, "gated_mlp").contiguous()
+        w12 = _saved(w12, (2 * H, D), dt, dev, "gated_mlp").contiguous()
+        w3 = _saved(w3, (O, H), dt, dev, "gated_mlp").contiguous()
+        kept = _saved(kept, (_bytes("iff_gated_mlp_kept_bytes", *sizes),), torch.uint8, dev, "gated_mlp").contiguous()
         dy, need = dy.contiguous(), ctx.needs_input_grad
         dx = x.new_empty((M, D)) if need[0] else None
         dw12 = x.new_empty((2 * H, D)) if need[1] else None
@@ -249,14 +270,17 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, residual, threshold, seed, seed_dev, offset):
         ctx.save_for_backward(seed_dev)           # (a seed tensor that changes before the backward pass is noticed by its version)
         ctx.how = (threshold, seed, offset)
+        ctx.seed_shape = None if seed_dev is None else seed_dev.shape
         return _dropout(x, residual, threshold, seed, seed_dev, offset)
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
         threshold, seed, offset = ctx.how
-        need = ctx.needs_input_grad
-        dx = _dropout(dy.contiguous(), None, threshold, seed, ctx.saved_tensors[0], offset) if need[0] else None
+        need, (seed_dev,) = ctx.needs_input_grad, ctx.saved_tensors
+        if seed_dev is not None:
+            seed_dev = _saved(seed_dev, ctx.seed_shape, torch.int64, dy.get_device(), "dropout")
+        dx = _dropout(dy.contiguous(), None, threshold, seed, seed_dev, offset) if need[0] else None
         return dx, dy if need[1] else None, None, None, None, None
 
 

@@ -1,0 +1,105 @@
+"""Calls of the trainable block operators that go through more of torch than the operator: hooks on saved tensors, forward-mode tangents,
+autocast, modules of all kinds under ``train_natively``."""
+import pytest
+import torch
+
+from iffnerf_amd import hip_block
+from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, normal
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+def copied():
+    """Saved tensors come back as dense copies, the way an offload or a compression hands them back."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t)
+
+
+def turned():
+    """... or with their axes the other way round in memory."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim()))))
+
+
+# ------------------------------------------------------------------------------------------------------------ hooks on saved tensors
+@pytest.mark.parametrize("hook", [copied, turned])
+def test_the_norms_backward_describes_the_tensor_it_is_handed(hook, monkeypatch):
+    """Without a GPU: the rows that the backward entry is told to read are the saved rows, inside the tensor (as_strided checks its bounds)."""
+    x = torch.arange(3 * 5 * 4, dtype=torch.float32).view(3, 5, 4)[:, 1:].requires_grad_(True)
+    seen = []
+
+    def record(name, t, *args):
+        if name == "iff_layer_norm_backward":
+            n0, n1, s0, s1, D = args[2:7]
+            assert args[0] == t.data_ptr()
+            seen.append(t.as_strided((n0, n1, D), (s0, s1, 1)).reshape(3, 4, 4).clone())
+
+    monkeypatch.setattr(hip_block, "_run", record)
+    w = torch.ones(4, requires_grad=True)
+    with hook():
+        y = hip_block._LayerNorm.apply(x, w, None, 1e-6)
+    torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert len(seen) == 1 and torch.equal(seen[0], x.detach())
+
+
+@pytest.mark.parametrize("change", [lambda t: t.half(), lambda t: t[None]], ids=["type", "shape"])
+def test_what_comes_back_as_something_else_is_refused(change, monkeypatch):
+    """Without a GPU: a hook that hands back another type or shape ends in an error, not in a launch."""
+    ran = []
+    monkeypatch.setattr(hip_block, "_run", lambda name, *a: ran.append(name))
+    x, w12, w3 = (torch.zeros(s, requires_grad=True) for s in ((3, 4), (12, 4), (5, 6)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        calls = [hip_block._LayerNorm.apply(x, torch.ones(4), None, 1e-6), hip_block._GatedMlp.apply(x, w12, None, w3, None, 0),
+                 hip_block._Dropout.apply(x, None, 100, 0, torch.zeros(1, dtype=torch.int64), 0)]
+    del ran[:]
+    for y in calls:
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(y, (x,), torch.ones_like(y))
+    assert not ran
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_gradients_under_hooks_on_saved_tensors(dev, dtype):
+    """save_on_cpu, copies and turned copies.  Norm over strided rows: the bounds of the plain call against 64 bits (a copy is aligned where
+    the view was not, so the backward pass may take another form and add in another order).  Feed-forward and dropout: the same bits."""
+    base = normal((3, 11, 48), 10, dtype)
+    w, b = normal((40,), 8, dtype, 0.2, 1.0), normal((40,), 9, dtype)
+    x, w12, b12, w3, b3, dy = make_mlp(20, 48, 80, 40, dtype, True, seed=50)
+    few, fdy = x[:3], dy[:3]
+    mlp = [t.requires_grad_(True) for t in (w12, b12, w3, b3)]
+    seed = torch.tensor([7], device=dev)
+
+    def more():
+        out = []
+        for inp, g in ((x, dy), (few, fdy)):
+            i = inp.detach().requires_grad_(True)
+            y = hip_block.gated_mlp(i, *mlp)
+            out += [y, *torch.autograd.grad(y, (i, *mlp), g)]
+        d = x.detach().requires_grad_(True)
+        y = hip_block.dropout(d, 0.3, seed)
+        return (*out, y, *torch.autograd.grad(y, (d,), torch.ones_like(y)))
+
+    views = [base[:, 1:, :40], base[:, :, 8:], base[:, ::2, 3:43], base[:, :, :40].transpose(0, 1), base[1, :, :40], base[:1, :, :40].expand(4, 11, 40)]
+    want = more()
+    for hook in (torch.autograd.graph.save_on_cpu, copied, turned):
+        for v in views:
+            with hook():
+                check_norm(v, w, b, 1e-6, normal(tuple(v.shape), 11, dtype))
+        with hook():
+            assert all(torch.equal(p, q) for p, q in zip(more(), want))
+
+
+@gpu
+def test_what_comes_back_on_another_device_is_refused(dev):
+    x, w12, _, w3, _, _ = make_mlp(4, 8, 8, 8, torch.float32, False)
+    x.requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        calls = [hip_block.layer_norm(x), hip_block.gated_mlp(x, w12, None, w3, None), hip_block.dropout(x, 0.5, torch.tensor([1], device=dev))]
+    for y in calls:
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(y, (x,), torch.ones_like(y))
