@@ -15,9 +15,11 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 from typing import Dict, Optional
 
 import torch
+import torch.fx
 import torch.nn.functional as F
 
 from . import _lib, hip_block
@@ -257,9 +259,20 @@ class _NativeLayerNorm(_NativeForward):
 
 
 class _NativeGatedMlp(_NativeForward):
+    def __init__(self, module):
+        super().__init__(module)
+        d = module.__dict__
+        self.children = tuple(module._modules.values())
+        self.others = tuple(c for c in self.children if c is not module.w12 and c is not module.w3)
+        self.attributes = tuple((k, v) for k, v in d.items() if k not in ("training", "forward") and not k.startswith("_"))
+        self.count = len(d) - ("forward" in d)
+
     def __call__(self, x):
         m = self.module
-        if not (_just_linear(m.w12) and _just_linear(m.w3)):      # a hook or a forward of their own, installed since: theirs to run
+        # what the module's forward was shown to compute holds for what it could go by then: hooks, children or attributes that came or
+        # changed since are the module's own forward's to deal with
+        if not (_just_linear(m.w12) and _just_linear(m.w3) and len(m.__dict__) == self.count + 1 and tuple(m._modules.values()) == self.children
+                and all(m.__dict__.get(k) is v for k, v in self.attributes) and all(c is None or _passes(c) for c in self.others)):
             return type(m).forward(m, x)
         return hip_block.gated_mlp(*_autocast(x, m.w12.weight, m.w12.bias, m.w3.weight, m.w3.bias))
 
@@ -289,22 +302,127 @@ def _runs(m, cls) -> bool:
     return isinstance(m, cls) and type(m).forward is cls.forward and isinstance(m.__dict__.get("forward"), (type(None), _NativeForward))
 
 
+def _unwatched(m) -> bool:
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def _just_linear(m) -> bool:
     """m is its weight and bias and nothing else: no hook would see, or change (weight norm), what a call that skips it computes."""
-    return _runs(m, torch.nn.Linear) and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+    return _runs(m, torch.nn.Linear) and _unwatched(m)
+
+
+def _passes(c) -> bool:
+    """A child beside ``w12`` and ``w3`` that a call may skip: SiLU, or the identity."""
+    return _unwatched(c) and ((_runs(c, torch.nn.SiLU) and not c.inplace) or _runs(c, torch.nn.Identity) or (_runs(c, torch.nn.Dropout) and c.p == 0.0))
+
+
+class _Watch(torch.fx.Tracer):
+    """Every child is a leaf; no operation is recorded outside the modes the trace began in (a ``no_grad`` or ``autocast`` inside the
+    forward is no operation itself)."""
+
+    def __init__(self):
+        super().__init__()
+        self.modes = self._modes()
+
+    @staticmethod
+    def _modes():
+        return (torch.is_grad_enabled(), torch.is_inference_mode_enabled(), torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))
+
+    def is_leaf_module(self, m, name):
+        return True
+
+    def create_node(self, *args, **kwargs):
+        if self._modes() != self.modes:
+            raise RuntimeError("an operation under modes of its own")
+        return super().create_node(*args, **kwargs)
+
+
+def _is_gated_silu_graph(m: torch.nn.Module, graph) -> bool:
+    """The traced operations are ``w3(silu(gate) * up)`` of ``[gate | up] = w12(x)``: each value is what it must be, and used once."""
+    half, value = m.w3.in_features, {}
+
+    def bound(node, *names):
+        return {**dict(zip(names, node.args)), **node.kwargs}
+
+    for n in graph.nodes:
+        users = 1
+        if n.op == "placeholder":
+            new = "x" if not value and not str(n.target).startswith("*") and not n.args else None
+        elif n.op == "call_module":
+            child, a = m.get_submodule(n.target), bound(n, "input")
+            of = value.get(a.pop("input", a.pop("x", None))) if len(a) == 1 else None
+            if child is m.w12:
+                new = "both" if of == "x" else None
+                users = 2 if len(n.users) == 2 else 1                  # (two slices, or one chunk)
+            elif child is m.w3:
+                new = "y" if of == "hidden" else None
+            elif _runs(child, torch.nn.SiLU):
+                new = "act" if of == "gate" else None
+            else:
+                new = of if _passes(child) else None
+        elif (n.op, n.target) in (("call_method", "chunk"), ("call_function", torch.chunk), ("call_method", "split"), ("call_function", torch.split)):
+            size = "chunks" if n.target in ("chunk", torch.chunk) else "split_size"
+            a = bound(n, "of", size, "dim")
+            a.setdefault("of", a.pop("input", a.pop("tensor", None)))
+            right = set(a) == {"of", size, "dim"} and a[size] == (2 if size == "chunks" else half) and a["dim"] == -1
+            new = "halves" if right and value.get(a["of"]) == "both" else None
+            users = 2
+        elif (n.op, n.target) == ("call_function", operator.getitem) and len(n.args) == 2 and not n.kwargs:
+            of, at = value.get(n.args[0]), n.args[1]
+            new = None
+            if of == "halves":
+                new = {0: "gate", 1: "up"}.get(at)
+            elif of == "both" and isinstance(at, tuple) and len(at) == 2 and at[0] is Ellipsis and isinstance(at[1], slice) and at[1].step is None:
+                new = {(None, half): "gate", (0, half): "gate", (half, None): "up", (half, 2 * half): "up"}.get((at[1].start, at[1].stop))
+        elif (n.op, n.target) == ("call_function", F.silu):
+            a = bound(n, "input", "inplace")
+            new = "act" if value.get(a.pop("input", None)) == "gate" and not a.pop("inplace", False) and not a else None
+        elif n.op in ("call_function", "call_method") and n.target in (operator.mul, torch.mul, "mul") and len(n.args) == 2 and not n.kwargs:
+            new = "hidden" if sorted(str(value.get(v)) for v in n.args if isinstance(v, torch.fx.Node)) == ["act", "up"] else None
+        elif n.op == "output":
+            return len(n.args) == 1 and isinstance(n.args[0], torch.fx.Node) and value.get(n.args[0]) == "y"
+        else:
+            new = None
+        if new is None or len(n.users) != users:
+            return False
+        value[n] = new
+    return False
+
+
+def _computes_gated_silu(m: torch.nn.Module) -> bool:
+    """What m's own forward does, by tracing it in training and evaluation, with and without gradients and autocast; a forward that cannot be
+    traced, takes more than its input, goes by the input's shape or values, or leaves something behind in the module does not count."""
+    before, training = dict(m.__dict__), m.training
+    cast, dtype = torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")
+    try:
+        torch.set_autocast_dtype("cuda", torch.bfloat16)
+        for mode in range(8):
+            m.training = bool(mode & 1)
+            torch.set_autocast_enabled("cuda", bool(mode & 2))
+            with torch.set_grad_enabled(bool(mode & 4)):
+                if not _is_gated_silu_graph(m, _Watch().trace(m)):
+                    return False
+        m.training = training
+        return list(m.__dict__) == list(before) and all(v is before[k] for k, v in m.__dict__.items())
+    except Exception:                            # (whatever a forward raises on a tensor that is none)
+        return False
+    finally:
+        torch.set_autocast_enabled("cuda", cast)
+        torch.set_autocast_dtype("cuda", dtype)
+        m.__dict__.clear()
+        m.__dict__.update(before)
 
 
 def _is_gated_silu(m: torch.nn.Module) -> bool:
-    """``w12`` and ``w3`` of matching widths, and nothing in the module that says more happens between them than SiLU."""
+    """``w12`` and ``w3`` of matching widths, nothing else that learns or keeps state, and a forward that is the gated SiLU block."""
     w12, w3 = getattr(m, "w12", None), getattr(m, "w3", None)
     if not (_just_linear(w12) and _just_linear(w3) and w12.out_features == 2 * w3.in_features):
         return False
-    if not isinstance(m.__dict__.get("forward"), (type(None), _NativeForward)):
+    if not isinstance(m.__dict__.get("forward"), (type(None), _NativeForward)) or m._parameters or m._buffers:
         return False
-    more = [c for name, c in m.named_children() if name not in ("w12", "w3")]
-    more += [m.__dict__[name] for name in ("act", "act_fn", "activation") if name in m.__dict__]
-    return all(c is None or c is F.silu or c == "silu" or isinstance(c, (torch.nn.SiLU, torch.nn.Identity))
-               or (isinstance(c, torch.nn.Dropout) and c.p == 0.0) for c in more)
+    if not all(c is None or c is w12 or c is w3 or _passes(c) for c in m.children()):
+        return False
+    return _computes_gated_silu(m)
 
 
 def _native_forward(m: torch.nn.Module):
@@ -325,8 +443,9 @@ def train_natively(module: torch.nn.Module) -> torch.nn.Module:
     pose_estimation/train.py:97-119 back-propagates through -- on ``hip_block``'s operators, forward and backward, and return THE SAME
     module.  As with ``serve_natively`` nothing is wrapped: classes, parameters and ``state_dict`` keys stay, one instance attribute
     ``forward`` per sub-module is installed.  The module then needs GPU tensors; values differ from stock torch by rounding, and a dropout's
-    mask comes from another generator (seeded by torch's).  A sub-module with a forward of its own, or a gated feed-forward that holds more than
-``w12``, ``w3`` and SiLU, is left as it is.  ``train_stock(module)`` removes it; without this call nothing changes."""
+    mask comes from another generator (seeded by torch's).  A norm or dropout with a forward of its own is left as it is, and so is every
+    feed-forward whose forward a symbolic trace does not show to be ``w3(silu(gate) * up)`` of ``[gate | up] = w12(x)``.
+    ``train_stock(module)`` removes it; without this call nothing changes."""
     for m in module.modules():
         f = _native_forward(m)
         if f is not None:

@@ -103,3 +103,173 @@ def test_what_comes_back_on_another_device_is_refused(dev):
     for y in calls:
         with pytest.raises(RuntimeError, match="came back as"):
             torch.autograd.grad(y, (x,), torch.ones_like(y))
+
+
+# ------------------------------------------------------------------------------------------------------------ train_natively
+class Ffn(torch.nn.Module):
+    """w12 and w3 of matching widths; what happens between them is the subclass's."""
+
+    def __init__(self, **more):
+        super().__init__()
+        self.w12, self.w3 = torch.nn.Linear(8, 12), torch.nn.Linear(6, 8)
+        for name, value in more.items():
+            setattr(self, name, value)
+
+
+def ffn(forward, **more):
+    return type("Its", (Ffn,), {"forward": forward})(**more)
+
+
+def chunked(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.silu(gate) * up)
+
+
+def gelu(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.gelu(gate) * up)
+
+
+def up_first(self, x):
+    up, gate = self.w12(x).chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.silu(gate) * up)
+
+
+def scaled_and_dropped(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.dropout(torch.nn.functional.silu(gate) * up * self.scale, 0.1, self.training))
+
+
+def dropped(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.dropout(torch.nn.functional.silu(gate) * up, self.drop, self.training))
+
+
+def own_nonlinearity(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    return self.w3(self.nonlinearity(gate) * up)
+
+
+def frozen_half(self, x):
+    with torch.no_grad():
+        both = self.w12(x)
+    gate, up = both.chunk(2, dim=-1)
+    return self.w3(torch.nn.functional.silu(gate) * up)
+
+
+def in_full_precision(self, x):
+    with torch.autocast("cuda", enabled=False):
+        return chunked(self, x)
+
+
+def training_noise(self, x):
+    h = chunked(self, x)
+    return h + 1.0 if self.training else h
+
+
+def residual(self, x):
+    return x + chunked(self, x)
+
+
+def clamped_when_long(self, x):
+    return chunked(self, x.clamp(-1, 1) if x.shape[0] > 100 else x)
+
+
+def other_axis(self, x):
+    gate, up = self.w12(x).chunk(2, dim=1)
+    return self.w3(torch.nn.functional.silu(gate) * up)
+
+
+def counting(self, x):
+    self.calls = getattr(self, "calls", 0) + 1
+    return chunked(self, x)
+
+
+def with_a_mask(self, x, mask=None):
+    return chunked(self, x if mask is None else x * mask)
+
+
+def twice(self, x):
+    gate, up = self.w12(x).chunk(2, dim=-1)
+    torch.nn.functional.silu(gate, inplace=True)
+    return self.w3(torch.nn.functional.silu(gate) * up)
+
+
+def w3_only(self, x):
+    return self.w3(x[..., :6])
+
+
+@pytest.mark.parametrize("forward,more", [
+    (gelu, {}), (up_first, {}), (scaled_and_dropped, {"scale": torch.nn.Parameter(torch.ones(6))}), (dropped, {"drop": 0.1}), (dropped, {"drop": 0.0}),
+    (own_nonlinearity, {"nonlinearity": torch.nn.functional.gelu}), (own_nonlinearity, {"nonlinearity": torch.nn.GELU()}),
+    (own_nonlinearity, {"nonlinearity": type("Other", (torch.nn.SiLU,), {"forward": lambda self, g: g})()}), (frozen_half, {}), (in_full_precision, {}),
+    (training_noise, {}), (residual, {}), (clamped_when_long, {}), (other_axis, {}), (counting, {}), (with_a_mask, {}), (twice, {}), (w3_only, {}),
+    (own_nonlinearity, {"nonlinearity": torch.nn.SiLU(inplace=True)}), (chunked, {"scale": torch.nn.Parameter(torch.ones(6))})],
+    ids=lambda v: v.__name__ if callable(v) else "-".join(v))
+def test_train_natively_goes_by_what_a_forward_computes(forward, more):
+    """Feed-forwards that look like a gated SiLU block from outside: left alone, their results their own, nothing in them touched."""
+    from iffnerf_amd import hip_vit
+    m = ffn(forward, **more)
+    state, x = dict(m.__dict__), torch.randn(2, 8, generator=torch.Generator().manual_seed(1))
+    modes = torch.is_grad_enabled(), torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")
+    torch.manual_seed(2)
+    with torch.no_grad():
+        want = m(x) if forward is not other_axis else None
+    if forward is counting:
+        del m.calls
+    for training in (True, False):
+        assert hip_vit.train_natively(m.train(training)) is m and m.training is training
+    m.train()
+    assert dict(m.__dict__).keys() == state.keys() and all(v is state[k] for k, v in m.__dict__.items())
+    assert modes == (torch.is_grad_enabled(), torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))
+    torch.manual_seed(2)
+    with torch.no_grad():
+        assert want is None or torch.equal(m(x), want)
+
+
+def sliced(self, x):
+    both = self.w12(x)
+    return self.w3(both[..., 6:] * torch.nn.functional.silu(both[..., :6]))
+
+
+def split(self, x):
+    gate, up = torch.split(self.w12(x), 6, dim=-1)
+    return self.w3(torch.nn.functional.silu(gate).mul(up))
+
+
+@pytest.mark.parametrize("forward,more", [(chunked, {}), (sliced, {}), (split, {}), (own_nonlinearity, {"nonlinearity": torch.nn.SiLU()}),
+                                          (own_nonlinearity, {"nonlinearity": torch.nn.functional.silu}), (chunked, {"note": "w"}), (chunked, {"unused": None})])
+def test_train_natively_takes_the_gated_silu_block(forward, more):
+    """However it is written; and a module that is changed afterwards runs its own forward again."""
+    from iffnerf_amd import hip_vit
+    m, x = ffn(forward, **more), torch.randn(2, 8, generator=torch.Generator().manual_seed(1))
+
+    def native():
+        try:
+            m(x)
+        except RuntimeError as e:
+            assert "no CPU path" in str(e)
+            return True
+        return False
+
+    hip_vit.train_natively(m)
+    assert "forward" in m.__dict__ and native() and not hip_vit.train_stock(m).__dict__.get("forward")
+    hip_vit.train_natively(m)
+    if "nonlinearity" in more:
+        m.nonlinearity = torch.nn.GELU() if isinstance(more["nonlinearity"], torch.nn.Module) else torch.nn.functional.gelu
+        assert not native() and torch.equal(m(x), forward(m, x))
+        m.nonlinearity = more["nonlinearity"]
+        assert native()
+    m.act = torch.nn.functional.gelu                                          # (an attribute that a forward may look for)
+    assert not native()
+    del m.act
+    assert native()
+    m.add_module("late", torch.nn.Identity())
+    assert not native()
+
+
+def test_train_natively_takes_the_stand_ins_own_block():
+    from iffnerf_amd import hip_vit
+    from iffnerf_amd.pose_estimation.backbone import SeededViTS14
+    m = hip_vit.train_natively(SeededViTS14(seed=3, dim=96, depth=2, heads=3, pretrain_grid=4, ffn="swiglu"))
+    assert all(isinstance(b.mlp.__dict__["forward"], hip_vit._NativeGatedMlp) for b in m.blocks)
