@@ -5,7 +5,7 @@ tensors (the training loop of the reference, pose_estimation/train.py:97-119, ba
 it through pose_estimation/backbone.py:12-14).  ``hip_vit.train_natively`` installs them on a backbone module.  fp32, bf16 and fp16;
 arithmetic and sums are fp32, a result is rounded once; every gradient is the same bits on every run.  Calls run on the current stream of
 the tensors' device, allocate through torch (so they can be captured into a hipGraph; take the gradients of a captured step with
-``torch.autograd.grad``) and raise ``RuntimeError`` for what they do not serve, CPU tensors among it.  First derivatives only.
+``torch.autograd.grad``) and raise ``RuntimeError`` for what they do not serve, CPU tensors and tensors with a forward-mode tangent among it.  First derivatives only.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import math
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -45,11 +46,20 @@ def _bytes(name: str, *sizes) -> int:
     return int(getattr(_lib.lib(), name)(*sizes))
 
 
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Inside a forward-mode level: the kernels would drop a tangent."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("layer_norm, gated_mlp and dropout have no forward-mode derivative: a tensor with a tangent cannot be an argument")
+
+
 def _first_derivative(backward):
     """``once_differentiable``, entered only where a second derivative could be asked for (autograd runs backward in grad mode then)."""
     guarded = once_differentiable(backward)
 
     def run(ctx, dy):
+        if forward_ad._current_level >= 0:
+            _no_tangents(dy)
         return guarded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
     return run
 
@@ -77,6 +87,8 @@ def _beside(t: torch.Tensor, x: torch.Tensor, name: str, shape, *types) -> torch
 
 
 def _trains(*tensors: Optional[torch.Tensor]) -> bool:
+    if forward_ad._current_level >= 0:
+        _no_tangents(*tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

@@ -273,3 +273,37 @@ def test_train_natively_takes_the_stand_ins_own_block():
     from iffnerf_amd.pose_estimation.backbone import SeededViTS14
     m = hip_vit.train_natively(SeededViTS14(seed=3, dim=96, depth=2, heads=3, pretrain_grid=4, ffn="swiglu"))
     assert all(isinstance(b.mlp.__dict__["forward"], hip_vit._NativeGatedMlp) for b in m.blocks)
+
+
+# ------------------------------------------------------------------------------------------------------------ forward-mode tangents
+@pytest.mark.parametrize("trains", [False, True])
+def test_tangents_are_refused(trains, monkeypatch):
+    """Without a GPU: a dual tensor in any place that has a derivative raises, whether or not it requires a gradient, and so does a dual
+    gradient; a forward-mode level alone changes nothing."""
+    from torch.autograd import forward_ad
+    ran = []
+    monkeypatch.setattr(hip_block, "_run", lambda name, *a: ran.append(name))
+    monkeypatch.setattr(hip_block, "_serves", lambda t, name: None)
+    x, w, w12, b12, w3, b3 = (torch.ones(s) for s in ((3, 4), (4,), (12, 4), (12,), (4, 6), (4,)))
+    for call, args in ((hip_block.layer_norm, (x, w, w)), (hip_block.gated_mlp, (x, w12, b12, w3, b3)),
+                       (lambda a, r: hip_block.dropout(a, 0.5, 1, residual=r), (x, x))):
+        for i in range(len(args)):
+            plain = [a.clone().requires_grad_(trains) for a in args]
+            with forward_ad.dual_level():
+                y = call(*plain)
+                assert len(ran) == 1
+                dual = list(plain)
+                dual[i] = forward_ad.make_dual(plain[i], torch.ones_like(plain[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                assert len(ran) == 1
+                if trains:
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        torch.autograd.grad(y, plain, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+                    assert len(ran) == 1
+            del ran[:]
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(hip_block.layer_norm, (x,), (x,))
+    assert not ran
