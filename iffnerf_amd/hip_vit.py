@@ -255,6 +255,8 @@ class _NativeForward:
 class _NativeLayerNorm(_NativeForward):
     def __call__(self, x):
         m = self.module
+        if x.shape[-1:] != m.normalized_shape:
+            raise RuntimeError(f"expected an input whose last axis is {m.normalized_shape[0]} wide (normalized_shape), got shape {tuple(x.shape)}")
         return hip_block.layer_norm(x, m.weight, m.bias, m.eps)
 
 

@@ -307,3 +307,21 @@ def test_tangents_are_refused(trains, monkeypatch):
     with pytest.raises(RuntimeError):
         torch.func.jvp(hip_block.layer_norm, (x,), (x,))
     assert not ran
+
+
+# ------------------------------------------------------------------------------------------------------------ what the modules around them do
+@pytest.mark.parametrize("affine", [True, False])
+def test_a_norm_of_another_width_is_refused(affine, monkeypatch):
+    """Without a GPU: as the module's own forward refuses it, with or without parameters."""
+    from iffnerf_amd import hip_vit
+    ran = []
+    monkeypatch.setattr(hip_block, "layer_norm", lambda x, *a: ran.append(x.shape))
+    m = torch.nn.LayerNorm(8, elementwise_affine=affine)
+    for x in (torch.zeros(2, 6), torch.zeros(2, 1), torch.zeros(8, 2), torch.zeros(())):
+        with pytest.raises(RuntimeError):
+            m(x)
+        with pytest.raises(RuntimeError, match="normalized_shape"):
+            hip_vit.train_natively(m)(x)
+        hip_vit.train_stock(m)
+    hip_vit.train_natively(m)(torch.zeros(2, 8))
+    assert ran == [(2, 8)]
