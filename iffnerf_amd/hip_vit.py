@@ -244,6 +244,13 @@ def _autocast(*tensors):
     return tuple(t if t is None or not t.is_floating_point() else t.to(dt) for t in tensors)
 
 
+def _in_fp32(*tensors):
+    """What an autocast region runs in fp32 gets 16-bit tensors as fp32 there (and answers in fp32); outside one, the tensors as they are."""
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    return tuple(t.float() if t is not None and t.dtype in (torch.float16, torch.bfloat16) else t for t in tensors)
+
+
 class _NativeForward:
     """The callable installed as a sub-module's ``forward`` by ``train_natively``.  It reads the module's own parameters at every call:
     optimizer steps, ``.to(...)`` and ``load_state_dict`` need nothing else."""
@@ -257,7 +264,7 @@ class _NativeLayerNorm(_NativeForward):
         m = self.module
         if x.shape[-1:] != m.normalized_shape:
             raise RuntimeError(f"expected an input whose last axis is {m.normalized_shape[0]} wide (normalized_shape), got shape {tuple(x.shape)}")
-        return hip_block.layer_norm(x, m.weight, m.bias, m.eps)
+        return hip_block.layer_norm(*_in_fp32(x, m.weight, m.bias), m.eps)
 
 
 class _NativeGatedMlp(_NativeForward):

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from iffnerf_amd import hip_block
-from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, normal
+from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, norm_reference, normal, within
 
 gpu = pytest.mark.gpu
 
@@ -325,3 +325,34 @@ def test_a_norm_of_another_width_is_refused(affine, monkeypatch):
         hip_vit.train_stock(m)
     hip_vit.train_natively(m)(torch.zeros(2, 8))
     assert ran == [(2, 8)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("par", [torch.float32, torch.bfloat16])
+def test_a_norm_under_autocast_answers_as_the_module_does(dev, dtype, par):
+    """fp32 whatever comes in, gradients in the leaves' types, within the bounds of an fp32 norm of the same values; outside the region the
+    input's type again."""
+    from iffnerf_amd import hip_vit
+    m = torch.nn.LayerNorm(40, eps=1e-6).to(dev, par)
+    with torch.no_grad():
+        m.weight.copy_(normal((40,), 1, par, 0.2, 1.0))
+        m.bias.copy_(normal((40,), 2, par, 0.3))
+    x, dy = normal((3, 7, 40), 3, dtype).requires_grad_(True), normal((3, 7, 40), 4)
+    leaves = (x, m.weight, m.bias)
+
+    def step():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = m(x)
+        return y, torch.autograd.grad(y, leaves, dy)
+
+    stock, sgrads = step()
+    hip_vit.train_natively(m)
+    y, grads = step()
+    assert y.dtype == stock.dtype == torch.float32 and [g.dtype for g in grads] == [g.dtype for g in sgrads]
+    want, lim = norm_reference(x.detach().float(), m.weight.detach(), m.bias.detach(), 1e-6, dy)
+    within(y.detach().reshape(-1, 40), want[0], lim[0], "y")
+    for g, w, e, name in zip(grads, want[1:], lim[1:], ("dx", "dw", "db")):
+        within(g, w, e, name)
+    if par == torch.float32:
+        assert m(x).dtype == dtype
