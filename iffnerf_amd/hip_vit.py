@@ -303,7 +303,10 @@ class _NativeDropAdd(_NativeForward):
         m = self.module
         if not (m.training and m.p > 0.0):
             return residual + branch
-        return hip_block.dropout(branch.to(residual.dtype), m.p, _fresh_seed(branch), residual=residual)
+        if residual.shape != branch.shape:                        # (a sum that broadcasts)
+            return residual + hip_block.dropout(branch, m.p, _fresh_seed(branch))
+        dt = torch.promote_types(residual.dtype, branch.dtype)
+        return hip_block.dropout(branch.to(dt), m.p, _fresh_seed(branch), residual=residual.to(dt))
 
 
 def _runs(m, cls) -> bool:

@@ -356,3 +356,29 @@ def test_a_norm_under_autocast_answers_as_the_module_does(dev, dtype, par):
         within(g, w, e, name)
     if par == torch.float32:
         assert m(x).dtype == dtype
+
+
+@gpu
+@pytest.mark.parametrize("rt", TYPES, ids=IDS)
+@pytest.mark.parametrize("bt", TYPES, ids=IDS)
+def test_the_sum_behind_a_dropout_is_in_the_wider_type(dev, rt, bt):
+    """residual + dropout(branch) of two types, and of shapes that broadcast: the type and shape of the module's own sum, its kept positions
+    to a rounding of the result, the residual exact where the branch is dropped, gradients in the leaves' types."""
+    from iffnerf_amd import hip_vit
+    from iffnerf_amd.pose_estimation.backbone import _DropAdd
+    m = _DropAdd(0.5)
+    for rs, bs in (((4, 33, 40), (4, 33, 40)), ((1, 40), (4, 33, 40)), ((4, 33, 40), (33, 40))):
+        r, b = normal(rs, 5, rt).requires_grad_(True), normal(bs, 6, bt, 3.0).requires_grad_(True)
+        stock = hip_vit.train_stock(m).train()(r, b)
+        hip_vit.train_natively(m)
+        y = m(r, b)
+        assert y.dtype == stock.dtype and y.shape == stock.shape
+        dy = normal(tuple(y.shape), 7, y.dtype)
+        dr, db = torch.autograd.grad(y, (r, b), dy)
+        assert dr.dtype == rt and db.dtype == bt and dr.shape == r.shape and db.shape == b.shape
+        if rs == bs:                                           # kept: db is 2 dy, 0 where dropped
+            keep = (db != 0).double()
+            assert 0.4 < float(keep.mean()) < 0.6 and torch.equal(dr, dy.to(rt))
+            want = r.detach().double() + 2.0 * b.detach().double() * keep
+            within(y.detach(), want, 2.0 ** -23 * (want.abs() + 2.0 * b.detach().double().abs()), "y")
+            assert torch.equal(y.detach()[keep == 0], r.detach().to(y.dtype)[keep == 0])
