@@ -148,6 +148,11 @@ class ViTHandle:
         return (tok, cls) if want_cls else tok
 
 
+def _dropouts():
+    from .pose_estimation.backbone import _DropAdd
+    return (torch.nn.Dropout, torch.nn.Dropout1d, torch.nn.Dropout2d, torch.nn.Dropout3d, torch.nn.AlphaDropout, torch.nn.FeatureAlphaDropout, _DropAdd)
+
+
 class _NativeForwardFeatures:
     """The callable installed as a backbone module's ``forward_features`` by ``serve_natively``.  It holds the module it serves (the
     module holds it in turn: an ordinary reference cycle) and the ``iff_vit`` handle built from the module's CURRENT parameters."""
@@ -191,6 +196,8 @@ class _NativeForwardFeatures:
             return self.stock(x, masks, *args, **kwargs)          # token masking / list inputs: DINOv2's training-side forms
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.module.parameters())):
             return self.stock(x)
+        if self.module.training and any(isinstance(m, _dropouts()) and m.p > 0.0 for m in self.module.modules()):
+            return self.stock(x)                                  # (the kernels drop nothing)
         if x.is_cuda and x.dim() == 4:
             # any input whose sides are multiples of the patch size is served, each grid by its own handle (the hub module accepts
             # them all: it interpolates its position table, and so does ViTHandle); grids beyond the kernels' token budget run the
@@ -210,8 +217,8 @@ def serve_natively(module: torch.nn.Module, grid=(16, 16), patch: int = 14, prec
     ``IdentificationModule`` built on it saves and strict-loads ``image_preprocessing_net.<backbone key>`` exactly as the reference
     does (train_eval_pose_est.py:59-66, pose_estimation/train.py:226).  Only the instance attribute ``forward_features`` is
     installed: no-grad inference on a GPU tensor goes through the HIP kernels (the handle is rebuilt when a parameter moves or
-    changes in place); with autograd enabled on a trainable backbone, with token masks or list inputs the module's own torch
-    forward runs.  ``precision``: see ``ViTHandle`` ("fp32": the reference's accuracy class, the default; "bf16": throughput).
+    changes in place); with autograd enabled on a trainable backbone, with a dropout at work (training mode), with token masks or list
+    inputs the module's own torch forward runs.  ``precision``: see ``ViTHandle`` ("fp32": the reference's accuracy class, the default; "bf16": throughput).
     ``restore_stock(module)`` removes it."""
     if precision not in PRECISIONS:
         raise RuntimeError(f"precision must be one of {sorted(PRECISIONS)} (got {precision!r})")
