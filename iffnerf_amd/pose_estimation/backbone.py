@@ -92,6 +92,12 @@ class _Block(torch.nn.Module):
         self.norm2, self.mlp, self.ls2 = torch.nn.LayerNorm(dim, eps=1e-6), {"mlp": _Mlp, "swiglu": _GatedMlp}[ffn](dim, mlp), _LayerScale(dim)
         self.add1, self.add2 = _DropAdd(drop), _DropAdd(drop)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ("add1", "add2"):                              # a module pickled before the sums were modules of their own
+            if name not in self._modules:
+                self.add_module(name, _DropAdd(0.0).train(self.training))
+
     def forward(self, x):
         x = self.add1(x, self.ls1(self.attn(self.norm1(x))))
         return self.add2(x, self.ls2(self.mlp(self.norm2(x))))

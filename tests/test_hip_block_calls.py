@@ -411,3 +411,18 @@ def test_a_served_backbone_in_training_mode_drops(monkeypatch):
         a, b = features(m), features(m)
         assert len(served) == 2 * native and ((a == "tokens") if native else not torch.equal(a, b))
         del served[:]
+
+
+def test_a_stand_in_pickled_whole_without_its_sums_still_loads():
+    """A module saved whole while its blocks had no add1 / add2: the same features after loading."""
+    import pickle
+    from iffnerf_amd.pose_estimation.backbone import SeededViTS14
+    m = SeededViTS14(seed=3, dim=96, depth=2, heads=3, pretrain_grid=4).eval()
+    x = torch.randn(1, 3, 56, 56, generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        want = m.forward_features(x)["x_prenorm"]
+        for b in m.blocks:
+            del b.add1, b.add2
+        old = pickle.loads(pickle.dumps(m))
+        assert torch.equal(old.forward_features(x)["x_prenorm"], want) and list(old.state_dict()) == list(m.state_dict())
+        assert not any(k.training for k in old.modules())
