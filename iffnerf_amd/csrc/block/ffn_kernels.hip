@@ -9,6 +9,7 @@
 // third rounding between dy and dx (against 64 bits: 2.1 roundings' worth instead of 1.4).
 #include "block_launch.h"
 #include "block_types.h"
+#include "ffn_plan.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -92,8 +93,6 @@ __device__ __forceinline__ void store4(T* o, const float v[4]) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     *reinterpret_cast<T4*>(o) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
 }
-
-__host__ __device__ constexpr int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Up to six matrices in one launch, job j from workgroup first[j] on: src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind
 // column C and behind row R of a half; 8 columns per thread
@@ -692,58 +691,6 @@ hipError_t tiles(Prod g, int splits, hipStream_t s) {
     k_ffn_product<T, AK, BK, EPI, WM, WN, MR, NR, NBUF><<<dim3((unsigned)(gm * gn), splits), 64 * WM * WN, 0, s>>>(g, (unsigned)gm, (unsigned)gn);
     return hipGetLastError();
 }
-// ---- which tiles, and how many shares of the k loop.  A round is one tile on every CU (two of the 128 x 128 ones); its time is modelled as
-// the k loop at the rate measured on full rounds (1.8 us per 64 k of a 256 x 256 tile; the smaller tiles move more operand bytes per
-// product: 5 % and 20 % on top) plus the epilogue's traffic at 4.5 GB/ms.  Two things decide between the shapes: how full the last round is
-// (a weight gradient of 8192 x 1536: one round of 256 x 192 tiles in 369 us, 0.75 rounds of 256 x 256 ones in 447 us), and the rows behind the last whole
-// tile (257 tokens per image leave 64 of them): as tiles of 256 they can cost a whole round, as a second launch of 128 x 128 tiles
-// about 6 us and their k loop.
-// A product with few tiles is bound by the latency of its steps instead: 0.85 us per 64 k of a 128 x 128 tile alone on its CU with two buffers,
-// less with four (then the tile has the CU to itself), and 64 x 64 tiles bring four times the workgroups.
-enum { SHAPE_256 = 0, SHAPE_192, SHAPE_128, SHAPE_128_DEEP, SHAPE_64, SHAPES };
-constexpr struct Shape { int bm, bn, slots_log2; double step; } kShape[SHAPES] = {     // step: us per 64 k of a round
-    {256, 256, 8, 1.8}, {256, 192, 8, 1.42}, {128, 128, 9, 1.08}, {128, 128, 8, 0.60}, {64, 64, 9, 0.45}};
-struct Plan { int shape, splits; int64_t main_rows; int rest_shape, rest_splits; };      // the rows behind main_rows go to a launch of their own
-
-// rows x N of C in one launch of `shape`, us (this runs at every call: nothing but the tile counts is divided per shape)
-struct Cost {
-    int64_t tiles[SHAPES]; double elements, traffic;
-    Cost(int64_t rows, int64_t N, double out_bytes) : elements((double)rows * N), traffic((double)rows * N * out_bytes / 4.5e6) {
-        for (int i = 0; i < SHAPES; ++i) tiles[i] = (rows + kShape[i].bm - 1) / kShape[i].bm * ((N + kShape[i].bn - 1) / kShape[i].bn);
-    }
-    double of(int shape, int splits, double steps) const {
-        const Shape& s = kShape[shape];
-        const int64_t rounds = (tiles[shape] * splits + (1 << s.slots_log2) - 1) >> s.slots_log2;
-        return (double)rounds * (steps * s.step + 3.0) + traffic + (splits > 1 ? 5.0 + elements * 4 * (splits + 1) / 4.5e6 : 0.0);
-    }
-};
-// out_bytes: what the epilogue moves per element of C; most: shares of the k loop that may be taken, each at least 256 deep
-inline Plan plan_tiles(int64_t M, int64_t N, int64_t K, double out_bytes, bool may_192, int most, bool may_rest = true) {
-    Plan best{SHAPE_128, 1, M, SHAPE_128, 1};
-    double least = 1e300, rest = 1e300;
-    const int64_t whole = may_rest && M % 256 ? M / 256 * 256 : 0;
-    const Cost all(M, N, out_bytes), behind(M - whole, N, out_bytes), front(whole, N, out_bytes);
-    const double steps_1 = (double)((K + 63) / 64);
-    int rest_shape = SHAPE_128, rest_splits = 1;
-    for (int z = 1; z <= most && (z == 1 || K >= 256 * (int64_t)z); z += z < 8 ? 1 : z < 16 ? 2 : 8) {      // 1 .. 8, 10 .. 16, 24 .. 64
-        const double steps = z == 1 ? steps_1 : (double)((K + 64 * z - 1) / (64 * z));
-        for (int shape = SHAPE_256; shape < SHAPES; ++shape) {
-            if (shape == SHAPE_192 && !may_192) continue;
-            const double t = all.of(shape, z, steps);
-            if (t < least) { least = t; best = {shape, z, M, SHAPE_128, 1}; }
-            if (!whole || shape < SHAPE_128 || z > 16) continue;
-            const double r = 6.0 + behind.of(shape, z, steps);
-            if (r < rest) { rest = r; rest_shape = shape; rest_splits = z; }
-        }
-    }
-    for (int shape = SHAPE_256; whole && shape <= SHAPE_192; ++shape) {
-        if (shape == SHAPE_192 && !may_192) continue;
-        const double two = front.of(shape, 1, steps_1) + rest;
-        if (two < least) { least = two; best = {shape, 1, whole, rest_shape, rest_splits}; }
-    }
-    return best;
-}
-
 template <class T, int AK, int BK, int EPI>
 hipError_t launch_shape(int shape, const Prod& g, int splits, hipStream_t s) {
     switch (shape) {
@@ -795,13 +742,8 @@ hipError_t rows_of(Work& w, Joins<T>& joins, Prod g, int64_t from, int shape, in
 }
 template <class T, int EPI>
 Plan product_plan(const Prod& g) {
-    constexpr double es = sizeof(T);
-    const int64_t K = g.K * (Mat<T>::P == 3 ? 6 : 1);
-    if (EPI == EPI_GATE) return plan_tiles(g.M, 2 * g.HP, K, (es + (g.p ? 8 : 0)) / 2, false, 1);
-    if (EPI == EPI_OUT) return plan_tiles(g.M, g.N, K, es, false, (int)std::max<int64_t>(1, std::min<int64_t>(16, g.K / 64)));
-    Plan p = plan_tiles(g.M, g.HP, K, 8 + 2 * es, false, 1);
-    if (p.rest_shape == SHAPE_64) p.rest_shape = SHAPE_128_DEEP;     // (one height of the waves' rows, that of the sums, per product)
-    return p;
+    constexpr int es = sizeof(T), pairs = Mat<T>::P == 3 ? 6 : 1;
+    return EPI == EPI_GATE ? gate_plan(g.M, g.HP, g.K, es, pairs, g.p) : EPI == EPI_DH ? dh_plan(g.M, g.HP, g.K, es, pairs) : rows_plan(g.M, g.N, g.K, es, pairs);
 }
 // a product over the rows of a batch
 template <class T, int AK, int BK, int EPI>
@@ -829,7 +771,7 @@ hipError_t product_of_pairs(Work& w, Joins<T>& joins, Prod g) {
 }
 template <class T>
 hipError_t weight_gradient(Work& w, Joins<T>& joins, Prod g, int64_t rows_out) {
-    const Plan p = plan_tiles(g.M, g.N, g.K * (Mat<T>::P == 3 ? 6 : 1), sizeof(T), true, (int)std::max<int64_t>(1, std::min<int64_t>(64, g.K / 256)), false);
+    const Plan p = weight_plan(g.M, g.N, g.K, sizeof(T), Mat<T>::P == 3 ? 6 : 1);
     g.rows_out = rows_out;
     if (p.splits > 1) g.part = (float*)w.take((size_t)p.splits * rows_out * g.N * 4);
     if (w.counting()) return hipSuccess;

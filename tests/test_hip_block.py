@@ -273,8 +273,8 @@ def test_gated_mlp_few_rows_are_exact_to_one_rounding(dev, M, D, H, O, act, bias
         within(g, want[1 + i], lim[1 + i], NAMES[i])
 
 
-# sizes at which each tile shape and each way of covering the rows is taken: whole 256 x 256 tiles, 256 x 192 ones in every layout, rows left to a
-# second launch (with and without shares of k), shares of a weight gradient, one round and several; one row more, one less
+# large sizes: whole 256 x 256 tiles, 256 x 192 ones of a weight gradient, a gate product in two launches, shares of a weight gradient, one round
+# and several; one row more, one less (tests/test_hip_block_plans.py holds sizes that take every form)
 @gpu
 @pytest.mark.parametrize("M,D,H,O,dtype", [
     (16384 + 64, 1536, 256, 192, torch.bfloat16), (8192 + 40, 192, 1024, 1536, torch.bfloat16), (16384, 192, 2048, 384, torch.float16),
