@@ -27,3 +27,14 @@ def pytest_collection_modifyitems(config, items):
 def golden():
     from tests import util
     return util.Golden()
+
+
+@pytest.hookimpl(tryfirst=True)
+def pytest_pyfunc_call(pyfuncitem):
+    """The tests of test_abi.py run in a thread each: iff_last_error() is a thread's, and what other tests' errors left is not theirs."""
+    if pyfuncitem.path.name != "test_abi.py":
+        return None
+    from concurrent.futures import ThreadPoolExecutor
+    with ThreadPoolExecutor(1) as one:
+        one.submit(pyfuncitem.obj, **{a: pyfuncitem.funcargs[a] for a in pyfuncitem._fixtureinfo.argnames}).result()
+    return True

@@ -426,3 +426,15 @@ def test_a_stand_in_pickled_whole_without_its_sums_still_loads():
         old = pickle.loads(pickle.dumps(m))
         assert torch.equal(old.forward_features(x)["x_prenorm"], want) and list(old.state_dict()) == list(m.state_dict())
         assert not any(k.training for k in old.modules())
+
+
+# ------------------------------------------------------------------------------------------------------------ the error text
+def test_the_suite_passes_in_any_order():
+    """The library keeps the text of a thread's last error; a test that asks for none must not go by what another one left."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-p", "no:cacheprovider", "tests/test_hip_block.py::test_c_entries_refuse_bad_arguments_without_a_gpu",
+                        "tests/test_abi.py::test_library_exports_every_declared_symbol"], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout[-2000:]
