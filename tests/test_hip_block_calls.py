@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from iffnerf_amd import hip_block
-from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, norm_reference, normal, within
+from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, norm_reference, normal, philox_bits, within
 
 gpu = pytest.mark.gpu
 
@@ -428,7 +428,27 @@ def test_a_stand_in_pickled_whole_without_its_sums_still_loads():
         assert not any(k.training for k in old.modules())
 
 
-# ------------------------------------------------------------------------------------------------------------ the error text
+# ------------------------------------------------------------------------------------------------------------ the generator, the error text
+def philox(c, k):
+    for _ in range(10):
+        p0, p1 = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(p1 >> 32) ^ c[1] ^ k[0], p1 & 0xFFFFFFFF, (p0 >> 32) ^ c[3] ^ k[1], p0 & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def test_the_generator_gives_the_published_answers():
+    """Philox 4x32-10 at all zeros, all ones and the digits of pi, and that the dropout tests' generator is the same function."""
+    ones, pi = [0xFFFFFFFF] * 6, [0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344, 0xA4093822, 0x299F31D0]
+    assert philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert philox(ones[:4], ones[4:]) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert philox(pi[:4], pi[4:]) == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    for seed, offset in ((0, 0), (2 ** 64 - 1, 2 ** 64 - 1), (5 << 33 | 9, 7 << 35 | 3)):
+        bits = philox_bits(24, seed, offset).tolist()
+        want = [w for b in range(3) for w in philox([b, 0, offset & 0xFFFFFFFF, offset >> 32], [seed & 0xFFFFFFFF, seed >> 32])]
+        assert [bits[2 * i] | bits[2 * i + 1] << 16 for i in range(12)] == want
+
+
 def test_the_suite_passes_in_any_order():
     """The library keeps the text of a thread's last error; a test that asks for none must not go by what another one left."""
     import os
