@@ -158,7 +158,8 @@ __device__ __attribute__((aligned(16))) const unsigned int g_zeros[4] = {0, 0, 0
 // 16 bytes per lane from `src` to LDS, lane-linear from byte `lds` on.  TR: as assembly -- behind the builtin the compiler drains the memory
 // queue before every transposed LDS read (it takes the two for aliases), which serialised the products with a k-strided operand (dW12 at
 // 16448 x 1536 x 4096: 745 against 369 us); beside plain reads the builtin is the faster form (F2: 219 against 245 us).  Nothing is
-// returned to a register; the waits are the kernel's own counted ones.  (Nothing else in these kernels uses m0.)
+// returned to a register; the waits are the kernel's own counted ones.  m0 is reserved: a clobber of it means nothing to the compiler, which
+// writes it right before each use of its own.  (That there is none in these kernels is tested on the built code.)
 template <bool TR>
 __device__ __forceinline__ void dma16(const char* src, uint32_t lds) {
     if constexpr (TR) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");

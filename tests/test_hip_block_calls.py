@@ -458,3 +458,31 @@ def test_the_suite_passes_in_any_order():
                         "tests/test_abi.py::test_library_exports_every_declared_symbol"], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                        capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout[-2000:]
+
+
+def test_nothing_beside_the_dma_uses_m0(tmp_path):
+    """The LDS-DMA written as assembly sets m0, a register that a statement cannot name as clobbered (the compiler keeps it out of its own
+    allocation and writes it right before each instruction that reads it).  In the built kernels with a k-strided operand every m0 belongs to
+    that statement: set, one s_nop, the DMA."""
+    import re
+    import shutil
+    import subprocess
+    from iffnerf_amd import build
+    build.build()
+    shutil.copy(build.CSRC + "/block/ffn_kernels.o", tmp_path / "k.o")
+    objdump = "/opt/rocm/llvm/bin/llvm-objdump"
+    subprocess.run([objdump, "--offloading", "k.o"], cwd=tmp_path, check=True, capture_output=True)
+    code, = tmp_path.glob("*gfx950")
+    text = subprocess.run([objdump, "-d", "--no-show-raw-insn", str(code)], check=True, capture_output=True, text=True).stdout
+    kernels = 0
+    for body in re.split(r"^[0-9a-f]+ <", text, flags=re.M)[1:]:
+        name, lines = body.split(">:", 1)
+        if "k_ffn_product" not in name or not re.search(r"k_ffn_productI(f|DF16b|DF16_)Li\dELi1E", name):          # <T, AK, BK = KS, ...>
+            continue
+        ops = [line.split("//")[0].split() for line in lines.splitlines() if line.split("//")[0].strip()]
+        uses = [i for i, op in enumerate(ops) if any("m0" == a.strip(",") for a in op[1:])]
+        for i in uses:
+            assert ops[i][0] == "s_mov_b32" and ops[i][1] == "m0," and ops[i + 1][0] == "s_nop" and ops[i + 2][0] == "global_load_lds_dwordx4", (name, ops[i])
+        assert uses and len(uses) == sum(op[0].startswith("global_load_lds") for op in ops)
+        kernels += 1
+    assert kernels == 39
