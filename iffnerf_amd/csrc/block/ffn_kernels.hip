@@ -49,9 +49,12 @@ template <class T>
 __device__ __forceinline__ void pieces(float v, typename Mat<T>::e out[Mat<T>::P]) {
     if constexpr (Mat<T>::P == 1) out[0] = (typename Mat<T>::e)v;
     else {
-        const bool ok = __builtin_isfinite(v);              // an infinity or a NaN travels in the first piece alone
-        const float a = ok ? trunc_bf16(v) : v, r = ok ? v - a : 0.0f, b = trunc_bf16(r);
-        out[0] = (__bf16)a; out[1] = (__bf16)b; out[2] = (__bf16)(r - b);
+        // An infinity is (the largest finite value, 0, infinity) with its sign: the third piece meets one other piece alone, the first of the
+        // other operand, which is 0 only where that operand is -- in the first piece it would meet pieces of 0 and end as a NaN.  The finite
+        // first piece brings another infinity's third to bear (inf x inf); all its products have the sign of the infinite one.  NaN likewise.
+        const bool ok = __builtin_isfinite(v);
+        const float a = ok ? trunc_bf16(v) : copysignf(__uint_as_float(0x7F7F0000u), v), r = ok ? v - a : 0.0f, b = trunc_bf16(r);
+        out[0] = (__bf16)a; out[1] = (__bf16)b; out[2] = (__bf16)(ok ? r - b : v);
     }
 }
 

@@ -250,7 +250,7 @@ def gated_mlp(x: torch.Tensor, w12: torch.Tensor, b12: Optional[torch.Tensor], w
     first -- the ``w12`` / ``w3`` layout of DINOv2's gated feed-forward), ``w3`` [O, H], biases [2 H] / [O] or None; one type and device.
     ``activation``: "silu" or "gelu" (exact).  Differentiable in all five.  The hidden activation is rounded to the type once (up to 8
     rows it has twice the type's precision); what the backward pass keeps next to it is fp32.  fp32 operands are multiplied as three bf16
-    pieces each, in fp32's accuracy; an infinite fp32 operand gives NaN."""
+    pieces each, in fp32's accuracy."""
     _serves(x, "gated_mlp: x")
     if activation not in _lib.ACTIVATIONS:
         raise RuntimeError(f"gated_mlp: activation must be one of {sorted(_lib.ACTIVATIONS)} (got {activation!r})")

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from iffnerf_amd import hip_block
-from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, norm_reference, normal, philox_bits, within
+from tests.test_hip_block import IDS, TYPES, check_norm, make_mlp, mlp_reference, norm_reference, normal, philox_bits, within
 
 gpu = pytest.mark.gpu
 
@@ -486,3 +486,47 @@ def test_nothing_beside_the_dma_uses_m0(tmp_path):
         assert uses and len(uses) == sum(op[0].startswith("global_load_lds") for op in ops)
         kernels += 1
     assert kernels == 39
+
+
+# ------------------------------------------------------------------------------------------------------------ infinities
+INF = float("inf")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES[:1], ids=IDS[:1])
+@pytest.mark.parametrize("M,D,H,O", [(1, 16, 24, 8), (3, 9, 13, 7), (8, 40, 24, 16), (12, 40, 24, 16), (70, 33, 66, 35)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_mlp_infinities_are_the_formulas(dev, M, D, H, O, act, dtype):
+    """An infinity in any operand, one of each sign, two that meet, one that meets a zero: every result is infinite, NaN or finite where the
+    formula in 64 bits is, with and without gradients, whatever the number of rows; the finite ones are within the usual bounds."""
+    places = [("x", (0, 1), INF), ("x", (M - 1, D - 1), -INF), ("w12", (2, 3), INF), ("w12", (H + 1, 0), -INF), ("w3", (1, 4), INF), ("w3", (O - 1, H - 1), -INF),
+              ("b12", (5,), INF), ("b12", (H + 2,), -INF), ("b3", (3,), INF), ("dy", (0, 2), INF), ("dy", (M - 1, 1), -INF), ("dy w3", (0, 1, 4), INF),
+              ("x w12", (0, 3, 2), INF), ("zero x w12", (3, 2), INF), ("zero w3 dy", (0, 1), INF), ("x", (0, 1), float("nan"))]
+    for where, at, value in places:
+        t = dict(zip(("x", "w12", "b12", "w3", "b3", "dy"), make_mlp(M, D, H, O, dtype, True, seed=400 + M)))
+        if where == "dy w3":
+            t["dy"][at[0], at[1]] = t["w3"][at[1], at[2]] = value
+        elif where == "x w12":
+            t["x"][at[0], at[1]] = t["w12"][at[2], at[1]] = value
+        elif where == "zero x w12":
+            t["x"][:, at[1]] = 0.0
+            t["w12"][at[0], at[1]] = value
+        elif where == "zero w3 dy":
+            t["w3"][at[1]] = 0.0
+            t["dy"][at] = value
+        else:
+            t[where][at] = value
+        names = ("x", "w12", "b12", "w3", "b3")
+        leaves = [t[n].requires_grad_(True) for n in names]
+        y = hip_block.gated_mlp(*leaves, activation=act)
+        got = (y.detach(), *torch.autograd.grad(y, leaves, t["dy"]))
+        want, lim = mlp_reference(*(t[n].detach() for n in names), act, t["dy"])
+        with torch.no_grad():
+            got, want, lim = (*got, hip_block.gated_mlp(*leaves, activation=act)), (*want, want[0]), (*lim, lim[0])
+        for g, w, e, name in zip(got, want, lim, ("y", "dx", "dw12", "db12", "dw3", "db3", "y without gradients")):
+            w = w.nan_to_num(nan=float("nan"), posinf=INF, neginf=-INF)
+            for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+                a, b = kind(g), kind(w)
+                assert torch.equal(a, b), f"{value} in {where}{at}: {name}: {kind.__name__} at {a.nonzero().tolist()[:4]}, the formula at {b.nonzero().tolist()[:4]}"
+            fine = w.isfinite() & e.isfinite()
+            within(g[fine], w[fine], e[fine], f"{value} in {where}{at}: {name}")
