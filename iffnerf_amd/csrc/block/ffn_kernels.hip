@@ -99,7 +99,8 @@ __device__ __forceinline__ void store4(T* o, const float v[4]) {
 
 // Up to six matrices in one launch, job j from workgroup first[j] on: src [halves x R][C] -> planes [P][halves x RP][CP], zeros behind
 // column C and behind row R of a half; 8 columns per thread
-struct PackJob { const void* src; void* dst; int64_t R, RP, C, CP, rows_out; int vec; };
+// With `finite` infinities and NaN leave as zeros.
+struct PackJob { const void* src; void* dst; int64_t R, RP, C, CP, rows_out; int vec, finite; };
 struct PackJobs { PackJob job[6]; unsigned first[7]; int n; };
 template <class T>
 __global__ void __launch_bounds__(256) k_ffn_pack(PackJobs jobs) {
@@ -124,6 +125,9 @@ __global__ void __launch_bounds__(256) k_ffn_pack(PackJobs jobs) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = r < j.R && c0 + i < j.C ? (float)s[i] : 0.0f;
         }
+        if (j.finite)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __builtin_isfinite(v[i]) ? v[i] : 0.0f;
         E8 o[P];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -564,10 +568,16 @@ __global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M
 
 // Sums of shares, every one a call leaves in one launch (a launch of its own costs each of them 5 us of GPU time and 4 of the host's): job j
 // from workgroup first[j] on.  Elements: out[i] = sum_z part[z][i] (+ bias of the column) in increasing z.  Columns (many shares, few sums):
-// 16 columns x 64 groups of shares per workgroup, a group in increasing order, the groups joined in order.
+// 16 columns x 64 groups of shares per workgroup, a group in increasing order, the groups joined in order.  PAIRS: elements whose odd shares
+// are products of what roundings left (product_of_pairs): where the sum is an infinity or a NaN, it is that of the even ones alone.
 enum { JOIN_ELEMENTS = 0, JOIN_COLUMNS = 1, JOIN_ELEMENTS4 = 2 };      // (the last: four at a time, where N and out allow it)
-struct JoinJob { const float* part; void* out; const void* bias; int64_t n, N; int Z, kind; };
+struct JoinJob { const float* part; void* out; const void* bias; int64_t n, N; int Z, kind; bool pairs; };
 struct JoinJobs { JoinJob job[6]; unsigned first[7]; int n; };
+__device__ __forceinline__ float even_shares(const JoinJob& j, int64_t i) {
+    float v = j.part[i];
+    for (int z = 2; z < j.Z; z += 2) v += j.part[z * j.n + i];
+    return v;
+}
 template <class T>
 __global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
     __shared__ float s[64][17];
@@ -587,6 +597,15 @@ __global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] += t[e];
             }
+            if (j.pairs && !(__builtin_isfinite(v[0]) & __builtin_isfinite(v[1]) & __builtin_isfinite(v[2]) & __builtin_isfinite(v[3])))
+#pragma unroll 1
+                for (int e = 0; e < 4; ++e) {                         // (one loop, not four: the code it sits in is 8 % slower with those)
+                    const float even = even_shares(j, i + e);
+                    v[0] = e == 0 && !__builtin_isfinite(v[0]) ? even : v[0];
+                    v[1] = e == 1 && !__builtin_isfinite(v[1]) ? even : v[1];
+                    v[2] = e == 2 && !__builtin_isfinite(v[2]) ? even : v[2];
+                    v[3] = e == 3 && !__builtin_isfinite(v[3]) ? even : v[3];
+                }
             if (bias)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] += (float)bias[i % j.N + e];
@@ -599,6 +618,7 @@ __global__ void __launch_bounds__(1024) k_ffn_join(JoinJobs jobs) {
         for (int64_t i = wg * (int64_t)1024 + threadIdx.x; i < j.n; i += (int64_t)wgs * 1024) {
             float v = j.part[i];
             for (int z = 1; z < j.Z; ++z) v += j.part[z * j.n + i];
+            if (j.pairs && !__builtin_isfinite(v)) v = even_shares(j, i);
             out[i] = (T)(bias ? v + (float)bias[i % j.N] : v);
         }
         return;
@@ -665,14 +685,15 @@ struct Packer {
     PackJobs jobs{};
     explicit Packer(Work& work) : w(work) {}
     // src [halves x R][C]; where the size is counted the copy is too (whether a start is 16-byte aligned must not change it).  `times`: the
-    // rows that many times over (16-bit types)
+    // rows that many times over (16-bit types), finite values alone after the first: what they are multiplied with there is what a rounding
+    // left, often 0, and an infinity's product is the first copy's to give
     Operand add(const void* src, int64_t halves, int64_t R, int64_t C, int times = 1) {
         const int64_t RP = halves > 1 ? pad8(R) : R, CP = pad8(C), rows = halves * RP;
         if (Mat<T>::P == 1 && CP == C && RP == R && times == 1 && !w.counting() && aligned16(src)) return {src, CP, rows * CP};
         char* dst = (char*)w.take(planes_bytes<T>(times * rows, CP));
         for (int i = 0; i < times && !w.counting() && rows; ++i) {
             const int64_t n = rows * CP / 8;
-            jobs.job[jobs.n] = {src, dst + i * planes_bytes<T>(rows, CP), R, RP, C, CP, rows, aligned16(src) && CP == C};
+            jobs.job[jobs.n] = {src, dst + i * planes_bytes<T>(rows, CP), R, RP, C, CP, rows, aligned16(src) && CP == C, i > 0};
             jobs.first[jobs.n + 1] = jobs.first[jobs.n] + (unsigned)std::min<int64_t>((n + 255) / 256, 4096);
             ++jobs.n;
         }
@@ -719,13 +740,13 @@ struct Joins {
         jobs.first[jobs.n + 1] = jobs.first[jobs.n] + (unsigned)wgs;
         ++jobs.n;
     }
-    void elements(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out) {
+    void elements(const float* part, int z, int64_t rows, int64_t N, const void* bias, void* out, bool pairs = false) {
         const int64_t n = rows * N;
         const bool four = N % 4 == 0 && aligned16(out);
         const int64_t per = four ? 4096 : 1024;
-        add({part, out, bias, n, N, z, four ? JOIN_ELEMENTS4 : JOIN_ELEMENTS}, std::min<int64_t>((n + per - 1) / per, 2048));
+        add({part, out, bias, n, N, z, four ? JOIN_ELEMENTS4 : JOIN_ELEMENTS, pairs}, std::min<int64_t>((n + per - 1) / per, 2048));
     }
-    void columns(const float* part, int64_t shares, int64_t N, void* out) { add({part, out, nullptr, N, N, (int)shares, JOIN_COLUMNS}, (N + 15) / 16); }
+    void columns(const float* part, int64_t shares, int64_t N, void* out) { add({part, out, nullptr, N, N, (int)shares, JOIN_COLUMNS, false}, (N + 15) / 16); }
     hipError_t go() {
         if (!jobs.n || w.counting()) return hipSuccess;
         k_ffn_join<T><<<jobs.first[jobs.n], 1024, 0, w.s>>>(jobs);
@@ -770,7 +791,7 @@ hipError_t product_of_pairs(Work& w, Joins<T>& joins, Prod g) {
     if (w.counting()) return hipSuccess;
     g.vec_out = g.N % 4 == 0;
     FFN_TRY((launch_shape<T, KC, BK, EPI_OUT>(p.shape, g, p.splits, w.s)));
-    joins.elements(g.part, 2 * p.splits, M, g.N, g.bias, g.out);
+    joins.elements(g.part, 2 * p.splits, M, g.N, g.bias, g.out, true);
     return hipSuccess;
 }
 template <class T>

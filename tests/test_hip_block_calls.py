@@ -493,7 +493,7 @@ INF = float("inf")
 
 
 @gpu
-@pytest.mark.parametrize("dtype", TYPES[:1], ids=IDS[:1])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("M,D,H,O", [(1, 16, 24, 8), (3, 9, 13, 7), (8, 40, 24, 16), (12, 40, 24, 16), (70, 33, 66, 35)])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gated_mlp_infinities_are_the_formulas(dev, M, D, H, O, act, dtype):
