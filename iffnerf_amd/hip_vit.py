@@ -274,7 +274,13 @@ class _NativeLayerNorm(_NativeForward):
         return hip_block.layer_norm(*_in_fp32(x, m.weight, m.bias), m.eps)
 
 
+def _same(a, b) -> bool:
+    return a is b or (type(a) is type(b) and isinstance(a, (int, float, str)) and a == b)      # (numbers are no longer the same object after pickling)
+
+
 class _NativeGatedMlp(_NativeForward):
+    count = -1                                                    # (pickled before a forward was looked at: the module's own runs)
+
     def __init__(self, module):
         super().__init__(module)
         d = module.__dict__
@@ -287,8 +293,8 @@ class _NativeGatedMlp(_NativeForward):
         m = self.module
         # what the module's forward was shown to compute holds for what it could go by then: hooks, children or attributes that came or
         # changed since are the module's own forward's to deal with
-        if not (_just_linear(m.w12) and _just_linear(m.w3) and len(m.__dict__) == self.count + 1 and tuple(m._modules.values()) == self.children
-                and all(m.__dict__.get(k) is v for k, v in self.attributes) and all(c is None or _passes(c) for c in self.others)):
+        if not (len(m.__dict__) == self.count + 1 and tuple(m._modules.values()) == self.children and _just_linear(m.w12) and _just_linear(m.w3)
+                and all(_same(m.__dict__.get(k), v) for k, v in self.attributes) and all(c is None or _passes(c) for c in self.others)):
             return type(m).forward(m, x)
         return hip_block.gated_mlp(*_autocast(x, m.w12.weight, m.w12.bias, m.w3.weight, m.w3.bias))
 

@@ -530,3 +530,27 @@ def test_gated_mlp_infinities_are_the_formulas(dev, M, D, H, O, act, dtype):
                 assert torch.equal(a, b), f"{value} in {where}{at}: {name}: {kind.__name__} at {a.nonzero().tolist()[:4]}, the formula at {b.nonzero().tolist()[:4]}"
             fine = w.isfinite() & e.isfinite()
             within(g[fine], w[fine], e[fine], f"{value} in {where}{at}: {name}")
+
+
+class Noted(Ffn):
+    forward = chunked
+
+
+def test_a_trained_backbone_survives_copies_and_pickles():
+    """Natively trained modules, copied and pickled: still native, on their own parameters; one pickled before forwards were looked at runs
+    its own."""
+    import copy
+    import pickle
+    from iffnerf_amd import hip_vit
+    x = torch.randn(2, 8, generator=torch.Generator().manual_seed(1))
+    m = hip_vit.train_natively(Noted(note="w", ratio=2.0 / 3.0, width=123456))
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            other(x)
+        assert other.__dict__["forward"].module is other
+        other.ratio = 0.5
+        assert torch.equal(other(x), chunked(other, x))
+    old = copy.deepcopy(m)
+    for name in ("children", "others", "attributes", "count"):
+        del old.__dict__["forward"].__dict__[name]
+    assert torch.equal(old(x), chunked(old, x))
