@@ -189,7 +189,7 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned gm, unsigned gn, u
 // slot c ^ (row / 2 & 7); a KS tile is rows of one k, chunk c in slot c ^ 4 (k & 3) (64 and 192 columns, whose rows are not whole
 // 256-byte bank rows: c ^ 2 (k & 2)), and its fragments are read transposed (ds_read_b64_tr_b16).  Both swizzles are applied to the
 // lanes' SOURCE addresses and keep the LDS reads free of bank conflicts.  What bounds it: the fill of LDS from L2 (a build that does
-// nothing else needs 0.6 - 0.8 of a launch) beside the matrix pipe (0.47 of F2's clocks at 16448 x 1536 x 4096, 242 us).  32-deep rings of
+// nothing else needs 0.6 - 0.8 of a launch) beside the matrix pipe (0.47 of F2's clocks at 16448 x 1536 x 4096, 217 us).  32-deep rings of
 // three to five buffers measured the same or slower, four waves of 128 x 128 17 % slower.
 template <class T, int AK, int BK, int EPI, int WM, int WN, int MR, int NR, int NBUF>
 __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2) k_ffn_product(Prod g, unsigned gm, unsigned gn) {
@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(64 * WM * WN, NBUF > 2 && MR * NR == 4 ? 1 : 2
 // At most 8 rows and no gradients (serving token by token): the weights are read once and that is all the time there is, so the products are
 // vector dot products -- a wave per RW rows of the weight matrix, its lanes over k, 16 bytes per load, fp32 sums joined across the lanes --
 // and not tiles of which 8 of 128 rows would be used.  GATE: RW / 2 hidden units, their gate and their up row; else RW outputs.  The hidden
-// activation stays fp32 between the two launches.  One token, 1536 x 4096 bf16: 7 + 4 us, 3.4 TB/s of weights.
+// activation stays fp32 between the two launches.  One token, 1536 x 4096 bf16: 6 + 4 us, 3.9 TB/s of weights (partly
+// from the Infinity Cache where they are read again at once).
 template <class T, int V, int MM, int RW, bool GATE, class TX, class TO>
 __global__ void __launch_bounds__(256) k_ffn_few(const TX* __restrict__ x, int M, int64_t K, const T* __restrict__ w, int64_t N, const T* __restrict__ bias,
                                                  int act, TO* __restrict__ out) {
