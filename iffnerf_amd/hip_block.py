@@ -5,7 +5,8 @@ tensors (the training loop of the reference, pose_estimation/train.py:97-119, ba
 it through pose_estimation/backbone.py:12-14).  ``hip_vit.train_natively`` installs them on a backbone module.  fp32, bf16 and fp16;
 arithmetic and sums are fp32, a result is rounded once; every gradient is the same bits on every run.  Calls run on the current stream of
 the tensors' device, allocate through torch (so they can be captured into a hipGraph; take the gradients of a captured step with
-``torch.autograd.grad``) and raise ``RuntimeError`` for what they do not serve, CPU tensors and tensors with a forward-mode tangent among it.  First derivatives only.
+``torch.autograd.grad``) and raise ``RuntimeError`` for what they do not serve, CPU tensors and tensors with a forward-mode tangent among
+it.  First derivatives only.
 """
 from __future__ import annotations
 

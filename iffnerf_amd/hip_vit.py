@@ -148,9 +148,12 @@ class ViTHandle:
         return (tok, cls) if want_cls else tok
 
 
-def _dropouts():
+def _drops(module: torch.nn.Module) -> bool:
+    """Something in ``module`` drops values in training mode."""
     from .pose_estimation.backbone import _DropAdd
-    return (torch.nn.Dropout, torch.nn.Dropout1d, torch.nn.Dropout2d, torch.nn.Dropout3d, torch.nn.AlphaDropout, torch.nn.FeatureAlphaDropout, _DropAdd)
+    nn = torch.nn
+    kinds = (nn.Dropout, nn.Dropout1d, nn.Dropout2d, nn.Dropout3d, nn.AlphaDropout, nn.FeatureAlphaDropout, _DropAdd)
+    return any(isinstance(m, kinds) and m.p > 0.0 for m in module.modules())
 
 
 class _NativeForwardFeatures:
@@ -196,7 +199,7 @@ class _NativeForwardFeatures:
             return self.stock(x, masks, *args, **kwargs)          # token masking / list inputs: DINOv2's training-side forms
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.module.parameters())):
             return self.stock(x)
-        if self.module.training and any(isinstance(m, _dropouts()) and m.p > 0.0 for m in self.module.modules()):
+        if self.module.training and _drops(self.module):
             return self.stock(x)                                  # (the kernels drop nothing)
         if x.is_cuda and x.dim() == 4:
             # any input whose sides are multiples of the patch size is served, each grid by its own handle (the hub module accepts
@@ -218,8 +221,8 @@ def serve_natively(module: torch.nn.Module, grid=(16, 16), patch: int = 14, prec
     does (train_eval_pose_est.py:59-66, pose_estimation/train.py:226).  Only the instance attribute ``forward_features`` is
     installed: no-grad inference on a GPU tensor goes through the HIP kernels (the handle is rebuilt when a parameter moves or
     changes in place); with autograd enabled on a trainable backbone, with a dropout at work (training mode), with token masks or list
-    inputs the module's own torch forward runs.  ``precision``: see ``ViTHandle`` ("fp32": the reference's accuracy class, the default; "bf16": throughput).
-    ``restore_stock(module)`` removes it."""
+    inputs the module's own torch forward runs.  ``precision``: see ``ViTHandle`` ("fp32": the reference's accuracy class, the default;
+    "bf16": throughput).  ``restore_stock(module)`` removes it."""
     if precision not in PRECISIONS:
         raise RuntimeError(f"precision must be one of {sorted(PRECISIONS)} (got {precision!r})")
     if not hasattr(type(module), "forward_features"):
@@ -275,7 +278,7 @@ class _NativeLayerNorm(_NativeForward):
 
 
 def _same(a, b) -> bool:
-    return a is b or (type(a) is type(b) and isinstance(a, (int, float, str)) and a == b)      # (numbers are no longer the same object after pickling)
+    return a is b or (type(a) is type(b) and isinstance(a, (int, float, str)) and a == b)      # (after pickling a number is another object)
 
 
 class _NativeGatedMlp(_NativeForward):

@@ -254,7 +254,8 @@ def test_train_natively_takes_the_gated_silu_block(forward, more):
 
     hip_vit.train_natively(m)
     assert "forward" in m.__dict__ and native() and not hip_vit.train_stock(m).__dict__.get("forward")
-    hip_vit.train_natively(m)
+    first = hip_vit.train_natively(m).__dict__["forward"]
+    assert hip_vit.train_natively(m).__dict__["forward"] is not first and native()                 # (installed again: looked at again)
     if "nonlinearity" in more:
         m.nonlinearity = torch.nn.GELU() if isinstance(more["nonlinearity"], torch.nn.Module) else torch.nn.functional.gelu
         assert not native() and torch.equal(m(x), forward(m, x))
